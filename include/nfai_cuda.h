@@ -395,6 +395,70 @@ int nfai_op_lm_head(nfai_ctx* ctx, const void* W, int dtype, const float* x, con
 int nfai_op_sample_top_p(nfai_ctx* c, const float* logits, uint32_t V, float temperature, float top_p, int top_k, float u,
                          uint32_t* token_out);
 
+/* ---- several answers to one prompt, one step of them at a time -----------------------------------------------------
+ * A host that asks for n answers to one prompt, or serves n chats behind one system prompt, keeps the prompt's keys and values
+ * once and gives every answer rows of its own behind them. nfai_op_gemm multiplies a batch of rows; these are the operators
+ * between the products. They have no counterpart in the reference, which serves one sequence.
+ *
+ * `stream`: NULL runs on the context's own stream and returns when the result is there, as every nfai_op_* above. Otherwise it is a
+ * cudaStream_t of the context's device (cudaStreamLegacy, the value 1, names the default stream): the work is put on that stream, the
+ * call returns at once and may be captured into a graph; scratch and buffers must then not be used by work that may run at the same
+ * time. The caller's current device stays what it was. */
+
+enum { NFAI_ROPE_PAIRS = 0 /* elements 2i and 2i+1, the reference's layout */, NFAI_ROPE_HALVES = 1 /* i and i + dims/2 */ };
+enum { NFAI_ROPE_PLAIN = 0, NFAI_ROPE_LINEAR = 1, NFAI_ROPE_BANDS = 2, NFAI_ROPE_YARN = 3 };
+
+/* Radians per position of the dims/2 pairs, in 64 bits, into freqs (host memory): f_i = base^(-2i/dims), changed for contexts longer
+ * than the `trained` one:
+ *   NFAI_ROPE_LINEAR  f_i / factor
+ *   NFAI_ROPE_BANDS   waves that turn more than b times within `trained` positions as they are, fewer than a times / factor, by
+ *                     degrees between (a < b, for example 1 and 4)
+ *   NFAI_ROPE_YARN    pairs up to the one that turns a times as they are, from the one that turns b times on / factor, by degrees
+ *                     between (a > b, for example 32 and 1); *magnitude = 0.1 ln(factor) + 1
+ * *magnitude (may be null) is 1 otherwise. Needs no context and no device.
+ * replaces: the table of TransformerBlock.cs:33-38 (plain, float32). */
+int nfai_rope_frequencies(uint32_t dims, double base, int scaling, double factor, double a, double b, uint32_t trained, double* freqs,
+                          float* magnitude);
+
+/* Queries, keys and values of a batch of tokens: the first `dims` elements of every query and key head turned by position * freq and
+ * multiplied by `magnitude`, the rest and the values as they are; queries into q_out [rows][qH*d], keys and values into rows of
+ * k_cache and v_cache [cache_rows][kvH*d]. x holds rows of x_stride elements (0: tightly packed), of which the first
+ * (qH + 2 kvH) * d are queries, keys and values, as nfai_op_gemm leaves them. x_dtype and out_dtype: NFAI_F32, NFAI_F16 or NFAI_BF16.
+ * positions[rows] and slots[rows] (the cache row of each; null: row r goes to cache row r) are device memory. A row whose slot is
+ * outside the cache (negative, for a padded batch) puts its keys and values nowhere. Slots of a call that are the same: it is not
+ * said whose rows stay. The angle is formed in 64 bits. qH or kvH may be 0. Outputs do not overlap x.
+ * replaces: RoPEShader (NFAI.Vulkan.Shaders/RoPEShader.cs:238-271) and the cache write of MatrixMultiplyShader.cs:286-287 for rows. */
+int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stride, uint32_t rows, uint32_t qH, uint32_t kvH, uint32_t d,
+                      uint32_t dims, int layout, const double* freqs, float magnitude, const int32_t* positions, const int32_t* slots,
+                      void* q_out, void* k_cache, void* v_cache, int out_dtype, uint64_t cache_rows, void* stream);
+
+/* Attention of one token of each of B sequences: out[b][h] = sum_t softmax_t(scale q[b][h] . k_t) v_t, where t runs over the `prefix`
+ * rows [prefix][kvH*d] that all share and over the first lens[b] of the sequence's own [B][capacity][kvH*d]. The shared rows are read
+ * once for all. q and out are [B][qH*d]; everything is of `dtype` (any of the three), sums and weights are float32 (weights of 16-bit
+ * caches are rounded to 16 bits for the product with the values). scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
+ * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
+ * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. What the rows behind
+ * lens[b] hold makes no difference. scratch (device memory, 256-byte aligned) is used until the work is done;
+ * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused).
+ * Where a wait inside the tensor-core kernel gives up, the rows become NaN, and a call without a stream returns NFAI_ERR_TIMEOUT. */
+int nfai_op_attn_shared(nfai_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,
+                        const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,
+                        uint32_t d, float scale, void* out, void* scratch, size_t scratch_bytes, void* stream);
+size_t nfai_op_attn_shared_scratch_bytes(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity);
+
+/* What a host wants of the next token, on the logits [rows][V] of every row, into out (the same buffer, or one that does not overlap):
+ *   c = how often the token stands in history[row][0 .. history_len[row]-1]
+ *   if c > 0:  x > 0 ? x / repetition[row] : x * repetition[row],  then  - frequency[row] * c - presence[row]
+ *   + the row's bias for the token: entries bias_start[row] .. bias_start[row+1]-1 of (bias_ids, bias); the last of several counts
+ *   -infinity where bit (token % 32) of word token / 32 of mask mask_rows[row] is 0; masks is [n_masks][(V + 31) / 32]; a row
+ *   whose mask_rows is not in 0 .. n_masks-1 (-1) is free; mask_rows null: row r has mask r
+ * All device memory. history rows are history_stride apart, history_len null means all of it, tokens of V and above count for nothing.
+ * Null: history (no penalties), repetition (1), frequency and presence (0); n_bias = 0 and n_masks = 0: none. */
+int nfai_op_logit_rules(nfai_ctx* ctx, const float* logits, uint32_t rows, uint32_t V, const uint32_t* history, uint32_t history_stride,
+                        const int32_t* history_len, const float* repetition, const float* frequency, const float* presence,
+                        const int32_t* bias_start, const uint32_t* bias_ids, const float* bias, uint32_t n_bias, const uint32_t* masks,
+                        uint32_t n_masks, const int32_t* mask_rows, float* out, void* stream);
+
 /* ---- multi-turn reuse --------------------------------------------------------------------------------------
  * nfai_prefill appends at the current position, so a second turn costs only its own tokens (the reference also keeps
  * growing one cache across turns, LlamaModel.cs:17,101-102, but never rewinds and overflows silently). A snapshot

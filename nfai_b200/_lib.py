@@ -38,7 +38,7 @@ class NfaiError(RuntimeError):
 
 
 # name -> (restype, argtypes); every symbol include/nfai_cuda.h declares
-_vp, _u32, _i, _f, _sz = C.c_void_p, C.c_uint32, C.c_int, C.c_float, C.c_size_t
+_vp, _u32, _i, _f, _d, _sz = C.c_void_p, C.c_uint32, C.c_int, C.c_float, C.c_double, C.c_size_t
 _pp = C.POINTER(C.c_void_p)
 SIGNATURES = {
     "nfai_version": (C.c_char_p, []),
@@ -105,6 +105,12 @@ SIGNATURES = {
     "nfai_op_attn_decode_static": (_i, [_vp, _vp, _vp, _vp, _i, _u32, _u32, _u32, _u32, _vp]),
     "nfai_op_gemm_f16": (_i, [_vp, _vp, _vp, _u32, _u32, _u32, _vp]),
     "nfai_op_gemm": (_i, [_vp, _vp, _vp, _i, _u32, _u32, _u32, _vp]),
+    "nfai_rope_frequencies": (_i, [_u32, _d, _i, _d, _d, _d, _u32, _vp, C.POINTER(_f)]),
+    "nfai_op_rope_rows": (_i, [_vp, _vp, _i, C.c_uint64, _u32, _u32, _u32, _u32, _u32, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i, C.c_uint64,
+                               _vp]),
+    "nfai_op_attn_shared": (_i, [_vp, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _vp, _i, _u32, _u32, _u32, _u32, _f, _vp, _vp, _sz, _vp]),
+    "nfai_op_attn_shared_scratch_bytes": (_sz, [_i, _u32, _u32, _u32, _u32, _u32, _u32]),
+    "nfai_op_logit_rules": (_i, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
     "nfai_op_lm_head": (_i, [_vp, _vp, _i, _vp, _vp, _f, _u32, _u32, _vp, _vp]),
 }
 
