@@ -15,6 +15,7 @@ using namespace shared_attn;
 
 constexpr int kST = 256;
 constexpr uint32_t kTK = 64;  // keys per tile
+constexpr uint32_t kSharedWalk = 512;  // shared rows from which on they are walked once for all
 
 __host__ __device__ constexpr uint32_t k_stride(uint32_t d) { return (d + 31) / 32 * 32 + 16; }  // two rows of a quarter-warp: other banks
 size_t any_smem_floats(uint32_t d, uint32_t rows) {
@@ -167,14 +168,24 @@ cudaError_t launch_own(cudaStream_t s, const SharedAttn& p, const SharedPlan& pl
 }  // namespace
 
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
-  (void)dtype;
   SharedPlan a;
   const uint32_t G = qH / kvH;
-  const uint64_t keys = (uint64_t)capacity + (a.pre_splits ? 0 : prefix);
-  a.rows = G <= 4 ? 4 : 8;
+  a.tensor = dtype != 0 && (d == 32 || d == 64 || d == 128);
+  const bool shared = dtype != 0 && (d == 64 || d == 128) && B >= 2 && prefix >= kSharedWalk;
+  if (shared) {
+    // two CTAs on every SM at once, each with 128 rows (sequence, head of the group) and as many tiles of keys as the others
+    const uint64_t groups = ((uint64_t)B * G + kPreRows - 1) / kPreRows * kvH;
+    const uint32_t tiles = (prefix + kPreTile - 1) / kPreTile;
+    uint64_t parts = 148 * 2 / groups;
+    parts = parts < 1 ? 1 : parts > kMaxPreSplits ? kMaxPreSplits : parts;
+    a.pre_tiles = (uint32_t)((tiles + parts - 1) / parts);
+    a.pre_splits = (tiles + a.pre_tiles - 1) / a.pre_tiles;
+  }
+  const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
+  a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
-  // CTAs for every SM three times over where the keys go so far (parts of 64 at least)
-  uint64_t parts = (148 * 3 + groups - 1) / groups;
+  // CTAs for every SM twice over (three times on the CUDA cores) where the keys go so far (parts of 64 at least)
+  uint64_t parts = (148 * (a.tensor && d == 128 ? 2 : 3) + groups - 1) / groups;
   if (parts > (keys + 63) / 64) parts = (keys + 63) / 64;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
@@ -195,11 +206,17 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
 }
 
 cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, const SharedPlan& plan) {
+  cudaError_t e = cudaSuccess;
   if (plan.own_splits > 1) {
     const uint32_t G = p.qH / p.kvH;
-    cudaError_t e = cudaMemsetAsync(p.tickets, 0, (size_t)p.B * p.kvH * ((G + plan.rows - 1) / plan.rows) * 4, s);
+    e = cudaMemsetAsync(p.tickets, 0, (size_t)p.B * p.kvH * ((G + plan.rows - 1) / plan.rows) * 4, s);
     if (e != cudaSuccess) return e;
   }
+  if (plan.pre_splits) {
+    e = launch_attn_shared_umma(s, dtype, p);
+    if (e != cudaSuccess) return e;
+  }
+  if (plan.tensor) return launch_attn_shared_mma(s, dtype, p, plan.rows);
   switch (dtype) {
     case 0: return launch_own<float>(s, p, plan);
     case 1: return launch_own<__half>(s, p, plan);

@@ -12,8 +12,10 @@
 namespace nfai {
 namespace shared_attn {
 
-constexpr uint32_t kMaxOwnSplits = 64;    // parts a sequence's keys are cut into
+constexpr uint32_t kMaxOwnSplits = 148;   // parts a sequence's keys are cut into
 constexpr uint32_t kMaxPreSplits = 148;   // parts of the shared rows
+constexpr uint32_t kPreRows = 128;        // (sequence, head of the group) of a CTA that walks the shared rows
+constexpr uint32_t kPreTile = 128;        // ... and its keys per tile
 constexpr uint32_t kSources = kMaxOwnSplits + kMaxPreSplits;
 constexpr uint32_t kMaxRows = 16;         // query heads per CTA
 
