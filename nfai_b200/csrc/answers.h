@@ -62,9 +62,9 @@ struct SharedAttn {
   float* pre_ml = nullptr;            // [pre_splits][kvH][B * G][2]
   float* own_o = nullptr;             // [own_splits][B * qH][d]
   float* own_ml = nullptr;            // [own_splits][B * qH][2]
-  uint32_t* tickets = nullptr;        // [B * kvH * head groups]
-  uint32_t pre_splits = 0, pre_tiles = 0;  // 0: the shared rows are walked like a sequence's own
+  uint32_t pre_splits = 0, pre_tiles = 0;  // parts of the shared rows, tiles of keys per CTA; 0: they are walked like a sequence's own
   uint32_t own_splits = 1;
+  bool joined = false;                // more than one partial result per row: they go to scratch and a last kernel joins them
   uint32_t* err = nullptr;            // device word of the context; may be null
 };
 // What the sizes alone decide: which kernels run, into how many parts, and what scratch they need.
@@ -72,7 +72,8 @@ struct SharedPlan {
   bool tensor = false;                // own rows on the warp-level tensor kernel (else CUDA cores)
   uint32_t rows = 8;                  // query heads per CTA there
   uint32_t pre_splits = 0, pre_tiles = 0, own_splits = 1;
-  size_t pre_o = 0, pre_ml = 0, own_o = 0, own_ml = 0, tickets = 0, total = 0;  // byte offsets
+  bool joined = false;
+  size_t pre_o = 0, pre_ml = 0, own_o = 0, own_ml = 0, total = 0;  // byte offsets
 };
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity);
 // the shared rows, partial results into pre_o and pre_ml; and everything else on the warp-level products

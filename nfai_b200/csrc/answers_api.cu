@@ -8,14 +8,15 @@
 
 namespace {
 
-// The context's device for the length of a call; the caller's current device is as it was afterwards.
+// The context's device for the length of a call; the caller's current device is as it was afterwards. Set even where it is the current
+// one already: in a thread that has not used the device yet, this is what makes its context current (tensor maps need one).
 struct OnDevice {
   int before = -1;
   cudaError_t err;
   explicit OnDevice(int device) {
     err = cudaGetDevice(&before);
-    if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
-    else if (err == cudaSuccess) before = -1;  // nothing to put back
+    if (err != cudaSuccess || before == device) before = -1;  // nothing to put back
+    if (err == cudaSuccess) err = cudaSetDevice(device);
   }
   ~OnDevice() {
     if (before >= 0) cudaSetDevice(before);
@@ -158,8 +159,8 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   p.B = B; p.qH = qH; p.kvH = kvH; p.d = d; p.out = out;
   p.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)d)) * 1.4426950408889634);
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
-  p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml); p.tickets = (uint32_t*)(base + plan.tickets);
-  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.err = c->dev_err;
+  p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
+  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.joined = plan.joined; p.err = c->dev_err;
   return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan));
 }
 

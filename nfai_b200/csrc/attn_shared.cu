@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p
     q[i] = a;  // (the queries have been used)
   }
   __syncthreads();
-  finish_rows<T, kST>(p, b, g, h0, nh, walk, blockIdx.y, blockIdx.x, q, d, m, l);
+  leave_rows<T, kST>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l);
 }
 
 template <typename T, int NR>
@@ -160,6 +160,125 @@ cudaError_t launch_any(cudaStream_t s, const SharedAttn& p) {
   const uint32_t hgroups = (p.qH / p.kvH + NR - 1) / NR;
   return launch_pdl(attn_shared_any_kernel<T, NR>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kST), smem, s, p.pre_splits != 0, p, hgroups);
 }
+// The join of partial results, a row of the output (sequence, query head) per WARPS warps: lanes have the parts' maxima and sums, then four
+// dimensions each, with the parts' rows asked for eight at a time.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(kST) attn_shared_join_kernel(const SharedAttn p) {
+  constexpr int kRows = kST / 32 / WARPS;
+  __shared__ float part_ml[kST / 32][2];
+  __shared__ __align__(16) float part_o[WARPS > 1 ? kST / 32 : 1][256];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WARPS, row = blockIdx.x * kRows + warp / WARPS, d = p.d;
+  pdl_wait();
+  const bool there = row < p.B * p.qH;
+  const uint32_t b = there ? row / p.qH : 0, h = row - b * p.qH, G = p.qH / p.kvH, g = h / G;
+  const Walk walk = walk_of(p, b, 0);
+  const bool busy = there && !walk.idle;
+  const uint32_t own = busy ? walk.parts : 0, n = busy ? own + p.pre_splits : 0;
+  const uint64_t BQ = (uint64_t)p.B * p.qH, R = (uint64_t)p.B * G, pre0 = (uint64_t)g * R + (uint64_t)b * G + (h - g * G);
+  auto at = [&](uint32_t i, const float*& o, const float*& ml) {  // part i
+    const uint64_t r = i < own ? (uint64_t)i * BQ + row : (uint64_t)(i - own) * p.kvH * R + pre0;
+    o = (i < own ? p.own_o : p.pre_o) + r * d;
+    ml = (i < own ? p.own_ml : p.pre_ml) + r * 2;
+  };
+  const uint32_t mine = n > sub ? (n - sub + WARPS - 1) / WARPS : 0;  // parts sub, sub + WARPS, ..
+  float M = -INFINITY, L = 0.f;
+  float4 acc[2] = {};
+  for (uint32_t k0 = 0; k0 < mine; k0 += 32) {
+    const uint32_t cnt = min(32u, mine - k0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < cnt) {
+      const float *o, *x;
+      at(sub + (k0 + lane) * WARPS, o, x);
+      ml = __ldcg(reinterpret_cast<const float2*>(x));
+    }
+    const float top = fmaxf(M, warp_max(ml.x)), ref = top == -INFINITY ? 0.f : top, before = exp2f(M - ref), f = exp2f(ml.x - ref);
+    M = top;
+    // (a part without weights: nothing of it counts, but a sum that is not a number does)
+    L = L * before + warp_sum(f != 0.f || ml.y != ml.y ? f * ml.y : 0.f);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      acc[u].x *= before; acc[u].y *= before; acc[u].z *= before; acc[u].w *= before;
+    }
+    for (uint32_t k = 0; k < cnt; k += 8) {
+      float4 v[8][2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float *o, *x;
+        at(sub + (k0 + min(k + j, cnt - 1)) * WARPS, o, x);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (u * 128 + lane * 4 < d) v[j][u] = __ldcg(reinterpret_cast<const float4*>(o + u * 128 + lane * 4));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = __shfl_sync(0xffffffffu, f, min(k + j, 31u));
+        if (k + j < cnt && w != 0.f) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (u * 128 + lane * 4 < d) {
+              acc[u].x = fmaf(w, v[j][u].x, acc[u].x); acc[u].y = fmaf(w, v[j][u].y, acc[u].y);
+              acc[u].z = fmaf(w, v[j][u].z, acc[u].z); acc[u].w = fmaf(w, v[j][u].w, acc[u].w);
+            }
+        }
+      }
+    }
+  }
+  if constexpr (WARPS > 1) {
+    if (lane == 0) {
+      part_ml[warp][0] = M;
+      part_ml[warp][1] = L;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (u * 128 + lane * 4 < d) *reinterpret_cast<float4*>(&part_o[warp][u * 128 + lane * 4]) = acc[u];
+    __syncthreads();
+    if (sub != 0) return;
+    const float first = M;
+    for (int w = 1; w < WARPS; ++w) M = fmaxf(M, part_ml[warp + w][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float f = exp2f(first - ref);
+    L = f != 0.f || L != L ? f * L : 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
+    }
+    for (int w = 1; w < WARPS; ++w) {
+      f = exp2f(part_ml[warp + w][0] - ref);
+      const float l = part_ml[warp + w][1];
+      if (f == 0.f && l == l) continue;
+      L = fmaf(f, l, L);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u * 128 + lane * 4 < d) {
+          const float4 v = *reinterpret_cast<const float4*>(&part_o[warp + w][u * 128 + lane * 4]);
+          acc[u].x = fmaf(f, v.x, acc[u].x); acc[u].y = fmaf(f, v.y, acc[u].y);
+          acc[u].z = fmaf(f, v.z, acc[u].z); acc[u].w = fmaf(f, v.w, acc[u].w);
+        }
+    }
+  }
+  if (!busy) return;
+  const float inv = p.prefix || walk.n ? 1.0f / L : 0.f;
+  T* const out = reinterpret_cast<T*>(p.out) + (uint64_t)row * d;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const uint32_t e = u * 128 + lane * 4;
+    if (e < d) {
+      store_as(out + e, acc[u].x * inv);
+      store_as(out + e + 1, acc[u].y * inv);
+      store_as(out + e + 2, acc[u].z * inv);
+      store_as(out + e + 3, acc[u].w * inv);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_join(cudaStream_t s, const SharedAttn& p) {
+  const uint32_t rows = p.B * p.qH;
+  if (p.pre_splits + p.own_splits > 8 && rows < 148 * 64)
+    return launch_pdl(attn_shared_join_kernel<T, 4>, dim3((rows + 1) / 2), dim3(kST), 0, s, true, p);
+  return launch_pdl(attn_shared_join_kernel<T, 1>, dim3((rows + 7) / 8), dim3(kST), 0, s, true, p);
+}
+
 template <typename T>
 cudaError_t launch_own(cudaStream_t s, const SharedAttn& p, const SharedPlan& plan) {
   return plan.rows == 4 ? launch_any<T, 4>(s, p) : launch_any<T, 8>(s, p);
@@ -173,19 +292,23 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   a.tensor = dtype != 0 && (d == 32 || d == 64 || d == 128);
   const bool shared = dtype != 0 && (d == 64 || d == 128) && B >= 2 && prefix >= kSharedWalk;
   if (shared) {
-    // two CTAs on every SM at once, each with 128 rows (sequence, head of the group) and as many tiles of keys as the others
-    const uint64_t groups = ((uint64_t)B * G + kPreRows - 1) / kPreRows * kvH;
+    // one CTA on every SM, each with two tiles of 128 rows (sequence, head of the group), or one tile twice, and as many keys as the others
+    const uint32_t row_tiles = (uint32_t)(((uint64_t)B * G + kPreRows - 1) / kPreRows), twice = row_tiles == 1;
+    const uint64_t groups = (uint64_t)(row_tiles + 1) / 2 * kvH;
     const uint32_t tiles = (prefix + kPreTile - 1) / kPreTile;
-    uint64_t parts = 148 * 2 / groups;
+    uint64_t parts = 148 / groups;
     parts = parts < 1 ? 1 : parts > kMaxPreSplits ? kMaxPreSplits : parts;
     a.pre_tiles = (uint32_t)((tiles + parts - 1) / parts);
+    // (one row tile: each of the CTA's two walks leaves a part of its own, and has a tile at least)
+    if (twice && a.pre_tiles < 2) a.pre_tiles = 2;
     a.pre_splits = (tiles + a.pre_tiles - 1) / a.pre_tiles;
+    if (twice) a.pre_splits *= 2;
   }
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
   a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
-  // CTAs for every SM twice over (three times on the CUDA cores) where the keys go so far (parts of 64 at least)
-  uint64_t parts = (148 * (a.tensor && d == 128 ? 2 : 3) + groups - 1) / groups;
+  // CTAs for every SM a few times over where the keys go so far (parts of 64 at least)
+  uint64_t parts = (148 * 4 + groups - 1) / groups;
   if (parts > (keys + 63) / 64) parts = (keys + 63) / 64;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
@@ -196,33 +319,25 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
     return at;
   };
   const uint64_t rows = (uint64_t)B * qH;
-  a.tickets = take(groups * 4);
+  a.joined = a.pre_splits || a.own_splits > 1;
   a.pre_ml = take(a.pre_splits * rows * 8);
-  a.own_ml = take(a.own_splits > 1 ? a.own_splits * rows * 8 : 0);
+  a.own_ml = take(a.joined ? a.own_splits * rows * 8 : 0);
   a.pre_o = take(a.pre_splits * rows * d * 4);
-  a.own_o = take(a.own_splits > 1 ? a.own_splits * rows * d * 4 : 0);
-  a.total = off;
+  a.own_o = take(a.joined ? a.own_splits * rows * d * 4 : 0);
+  a.total = off > 256 ? off : 256;  // (one part per row needs none: a size is never 0)
   return a;
 }
 
 cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, const SharedPlan& plan) {
   cudaError_t e = cudaSuccess;
-  if (plan.own_splits > 1) {
-    const uint32_t G = p.qH / p.kvH;
-    e = cudaMemsetAsync(p.tickets, 0, (size_t)p.B * p.kvH * ((G + plan.rows - 1) / plan.rows) * 4, s);
-    if (e != cudaSuccess) return e;
-  }
   if (plan.pre_splits) {
     e = launch_attn_shared_umma(s, dtype, p);
     if (e != cudaSuccess) return e;
   }
-  if (plan.tensor) return launch_attn_shared_mma(s, dtype, p, plan.rows);
-  switch (dtype) {
-    case 0: return launch_own<float>(s, p, plan);
-    case 1: return launch_own<__half>(s, p, plan);
-    case 2: return launch_own<__nv_bfloat16>(s, p, plan);
-    default: return cudaErrorInvalidValue;
-  }
+  if (plan.tensor) e = launch_attn_shared_mma(s, dtype, p, plan.rows);
+  else e = dtype == 0 ? launch_own<float>(s, p, plan) : dtype == 1 ? launch_own<__half>(s, p, plan) : launch_own<__nv_bfloat16>(s, p, plan);
+  if (e != cudaSuccess || !p.joined) return e;
+  return dtype == 0 ? launch_join<float>(s, p) : dtype == 1 ? launch_join<__half>(s, p) : launch_join<__nv_bfloat16>(s, p);
 }
 
 }  // namespace nfai

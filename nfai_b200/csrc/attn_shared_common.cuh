@@ -3,7 +3,7 @@
 // A partial result of one query head is (o[d], m, l): m the largest score (base 2) among its keys, l = sum 2^(s - m), o = sum 2^(s - m) v.
 // No keys, or keys whose scores are all -infinity: m = -infinity, l = 0. Several are joined as
 //   M = max m_i,  out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
-// in the order of their index, whichever CTA does it: the result does not depend on who came last.
+// in an order that follows from their indices alone: the same call gives the same bits.
 #pragma once
 #include "answers.h"
 #include "common.cuh"
@@ -13,11 +13,9 @@ namespace nfai {
 namespace shared_attn {
 
 constexpr uint32_t kMaxOwnSplits = 148;   // parts a sequence's keys are cut into
-constexpr uint32_t kMaxPreSplits = 148;   // parts of the shared rows
+constexpr uint32_t kMaxPreSplits = 148;   // CTAs that the shared rows are divided among
 constexpr uint32_t kPreRows = 128;        // (sequence, head of the group) of a CTA that walks the shared rows
 constexpr uint32_t kPreTile = 128;        // ... and its keys per tile
-constexpr uint32_t kSources = kMaxOwnSplits + kMaxPreSplits;
-constexpr uint32_t kMaxRows = 16;         // query heads per CTA
 
 __device__ __forceinline__ float s_ex2(float x) {
   float y;
@@ -42,9 +40,11 @@ __device__ __forceinline__ Walk walk_of(const SharedAttn& p, uint32_t b, uint32_
   w.t1 = min(w.n, w.t0 + chunk);
   return w;
 }
-// A CTA's way out before it has seen the shared rows' parts: the next kernel in the stream counts on this grid to end behind theirs.
+// A CTA's way out. The join starts when this grid has ended and counts on the walk of the shared rows to have ended too: the last CTA
+// sees to that.
 __device__ __forceinline__ void leave(const SharedAttn& p) {
-  if (p.pre_splits) pdl_wait();
+  if (p.joined) pdl_launch_dependents();
+  if (p.pre_splits && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) pdl_wait();
 }
 // Offset of key t of sequence b: in the shared rows, or in the sequence's own (`own` set).
 __device__ __forceinline__ uint64_t key_row(const SharedAttn& p, uint32_t b, uint32_t t, bool& own) {
@@ -54,76 +54,30 @@ __device__ __forceinline__ uint64_t key_row(const SharedAttn& p, uint32_t b, uin
 }
 
 // Everything a CTA does behind its walk: rows[j][d] (stride ld), m[j], l[j] of its query heads h0 .. h0 + nh - 1 are in shared memory,
-// all of it written and synchronised.
+// all of it written and synchronised. The only part of a sequence is its result, others go to scratch for the join.
 template <typename T, int THREADS>
-__device__ __forceinline__ void finish_rows(const SharedAttn& p, uint32_t b, uint32_t g, uint32_t h0, uint32_t nh, const Walk& w,
-                                            uint32_t split, uint32_t ticket, const float* rows, uint32_t ld, const float* m,
-                                            const float* l) {
-  __shared__ float weight[kMaxRows][kSources];
-  __shared__ float inverse[kMaxRows];
-  __shared__ uint32_t last;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = p.d, G = p.qH / p.kvH, BQ = p.B * p.qH;
-  const uint32_t row0 = b * p.qH + h0;
-  if (w.parts > 1) {
-    for (uint32_t i = tid; i < nh * d; i += THREADS) {
-      const uint32_t j = i / d, e = i - j * d;
-      p.own_o[((uint64_t)split * BQ + row0 + j) * d + e] = rows[j * ld + e];
+__device__ __forceinline__ void leave_rows(const SharedAttn& p, uint32_t b, uint32_t h0, uint32_t nh, const Walk& w, uint32_t split,
+                                           const float* rows, uint32_t ld, const float* m, const float* l) {
+  const uint32_t tid = threadIdx.x, d = p.d, d4 = d / 4, row0 = b * p.qH + h0;
+  if (p.joined) {
+    const uint64_t at = (uint64_t)split * p.B * p.qH + row0;
+    for (uint32_t i = tid; i < nh * d4; i += THREADS) {
+      const uint32_t j = i / d4, e = (i - j * d4) * 4;
+      *reinterpret_cast<float4*>(p.own_o + (at + j) * d + e) = *reinterpret_cast<const float4*>(rows + j * ld + e);
     }
-    if (tid < nh) *reinterpret_cast<float2*>(p.own_ml + ((uint64_t)split * BQ + row0 + tid) * 2) = make_float2(m[tid], l[tid]);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) last = atomicAdd(p.tickets + ticket, 1u) == w.parts - 1 ? 1u : 0u;
-    __syncthreads();
-    if (!last) return leave(p);
-    __threadfence();
+    if (tid < nh) *reinterpret_cast<float2*>(p.own_ml + (at + tid) * 2) = make_float2(m[tid], l[tid]);
+    leave(p);
+    return;
   }
-  if (p.pre_splits) pdl_wait();  // the parts of the shared rows are there
-  const uint32_t own = w.parts, n = own + p.pre_splits;
-  auto pre_row = [&](uint32_t i, uint32_t j) { return ((uint64_t)i * p.kvH + g) * ((uint64_t)p.B * G) + (uint64_t)b * G + (h0 - g * G) + j; };
-  for (uint32_t j = warp; j < nh; j += THREADS / 32) {
-    auto ml = [&](uint32_t i) {
-      if (i >= own) return __ldcg(reinterpret_cast<const float2*>(p.pre_ml + pre_row(i - own, j) * 2));
-      if (own > 1) return __ldcg(reinterpret_cast<const float2*>(p.own_ml + ((uint64_t)i * BQ + row0 + j) * 2));
-      return make_float2(m[j], l[j]);
-    };
-    float M = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) {
-      const float2 a = ml(i);
-      weight[j][i] = a.x;
-      M = fmaxf(M, a.x);
-    }
-    M = warp_max(M);
-    float L = 0.f;
-    for (uint32_t i = lane; i < n; i += 32) {
-      const float f = weight[j][i] == -INFINITY ? 0.f : exp2f(weight[j][i] - M);
-      weight[j][i] = f;
-      const float li = ml(i).y;
-      if (f != 0.f || li != li) L = fmaf(f, li, L);
-    }
-    L = warp_sum(L);
-    if (lane == 0) inverse[j] = 1.0f / L;
-  }
-  __syncthreads();
-  const bool nothing = p.prefix == 0 && w.n == 0;
   T* const out = reinterpret_cast<T*>(p.out) + (uint64_t)row0 * d;
-  for (uint32_t i = tid; i < nh * d; i += THREADS) {
-    const uint32_t j = i / d, e = i - j * d;
-    float acc = 0.f;
-    if (own > 1) {
-#pragma unroll 4
-      for (uint32_t k = 0; k < own; ++k) {
-        const float f = weight[j][k], v = __ldcg(p.own_o + ((uint64_t)k * BQ + row0 + j) * d + e);
-        acc = f != 0.f ? fmaf(f, v, acc) : acc;
-      }
-    } else if (weight[j][0] != 0.f) {
-      acc = weight[j][0] * rows[j * ld + e];
-    }
-#pragma unroll 4
-    for (uint32_t k = 0; k < p.pre_splits; ++k) {
-      const float f = weight[j][own + k], v = __ldcg(p.pre_o + pre_row(k, j) * d + e);
-      acc = f != 0.f ? fmaf(f, v, acc) : acc;
-    }
-    store_as(out + i, nothing ? 0.f : acc * inverse[j]);
+  for (uint32_t i = tid; i < nh * d4; i += THREADS) {
+    const uint32_t j = i / d4, e = (i - j * d4) * 4;
+    const float f = w.n ? 1.0f / l[j] : 0.f;  // (no keys at all: zeros; none with a weight: 0 * infinity)
+    const float4 v = *reinterpret_cast<const float4*>(rows + j * ld + e);
+    store_as(out + j * d + e, v.x * f);
+    store_as(out + j * d + e + 1, v.y * f);
+    store_as(out + j * d + e + 2, v.z * f);
+    store_as(out + j * d + e + 3, v.w * f);
   }
 }
 

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p
     }
   }
   __syncthreads();
-  finish_rows<T, kMT>(p, b, g, h0, nh, walk, split, blockIdx.x, rows, PL, M, L);
+  leave_rows<T, kMT>(p, b, h0, nh, walk, split, rows, PL, M, L);
 }
 
 template <typename T, int D, int ROWS>

@@ -1,18 +1,19 @@
 // The shared rows, once for every sequence: 16-bit types, heads of 64 and 128, on the 5th-generation tensor cores.
 //
-// The query heads of a KV head and the sequences are one list of rows (row = sequence * G + head of the group). A CTA owns 128 of
-// them, one accumulator lane each, and walks a part of the keys in tiles of 128:
-//   warp 8   K and V tiles by TMA into a ring of 128-byte swizzled slots, in the order in which they are multiplied
-//   warp 9   one lane issues S = Q K^T and O += P V (P in tensor memory, V as it lies: its rows run along N)
-//   warps 0-7  softmax, two threads to a row (64 keys each): weights back into tensor memory as the 16-bit operand of the second
-//            product, their float32 sums kept; at the end (sums of weighted values, maximum, sum of weights) go to scratch, and the kernel of
-//            the own rows joins them.
-// Every key is fetched once per 128 rows (the CTAs of further rows find it in L2). With fewer rows than 128 the warps of rows that are
-// not there leave the exponentials out. Scores are products of the 16-bit queries as they are; the scale goes into the exponent's
-// multiply-add. A row's sums are rescaled only when its maximum has grown by more than 2^8 since the last time.
+// The query heads of a KV head and the sequences are one list of rows (row = sequence * G + head of the group). A CTA has two streams of
+// 128 rows each, one accumulator lane a row, and walks a part of the keys in tiles of 128. With more than 128 rows the streams are
+// neighbouring row tiles on the same keys, which are then fetched once for 256 rows; with fewer they are the same rows on every second
+// tile of keys, and leave two parts for the join. While one stream forms its weights the tensor pipe works for the other:
+//   warp 16  K and V tiles by TMA into a ring of 128-byte swizzled slots, in the order in which they are multiplied
+//   warp 17  one lane issues S(0), S(1), then for every unit (stream, tile) u: O += P(u) V, S(u + 2) = Q K^T, with P in tensor memory where S(u)
+//            was and V as it lies (its rows run along N)
+//   warps 0-7 and 8-15  softmax of a stream, two threads to a row (64 keys each): weights back into tensor memory as the 16-bit
+//            operand of the second product, their float32 sums kept; at the end (sums of weighted values, maximum, sum of weights) go
+//            to scratch, and attn_shared_join_kernel joins them with those of the own rows.
+// Warps whose rows are not there leave the exponentials out. Scores are products of the 16-bit queries as they are; the scale goes
+// into the exponent's multiply-add. A row's sums are rescaled only when its maximum has grown by more than 2^8 since the last time.
 #include <type_traits>
 
-#include "attn_phases.h"
 #include "attn_shared_common.cuh"
 #include "umma.cuh"
 
@@ -24,19 +25,32 @@ using namespace umma;
 using shared_attn::kPreRows;
 using shared_attn::kPreTile;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 576;
 constexpr float kGrowth = 8.0f;
-using Values = ValuePhases<1>;
 
 template <int D>
 struct PreSmem {
   static constexpr uint32_t kTile = kPreTile * D * 2;
-  static constexpr uint32_t kSlots = D == 64 ? 5 : 2;  // two CTAs on an SM
-  static constexpr uint32_t kQ = kPreRows * D * 2;
-  static constexpr uint32_t kBarOff = kQ + kSlots * kTile;
-  static constexpr uint32_t kSwapOff = kBarOff + 256;
-  static constexpr uint32_t kTotal = kSwapOff + 2 * kPreRows * 4 + 1024;
+  static constexpr uint32_t kSlots = D == 64 ? 12 : 5;
+  static constexpr uint32_t kQ = kPreRows * D * 2;  // of one stream
+  static constexpr uint32_t kRing = 2 * kQ;
+  static constexpr uint32_t kBarOff = kRing + kSlots * kTile;
+  static constexpr uint32_t kSwapOff = kBarOff + 256;  // [stream][half][row]: maxima of the halves of a row, later their sums
+  static constexpr uint32_t kTotal = kSwapOff + 4 * kPreRows * 4;
 };
+static_assert(PreSmem<64>::kTotal <= 232448 && PreSmem<128>::kTotal <= 232448, "shared memory of a CTA");
+
+// Bounded waits as in umma.cuh; the limit is counted in cycles, whose counter is read in a few of them (the nanosecond timer takes
+// longer than some of these waits).
+constexpr long long kWaitCycles = 2000000000ll;
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+  if (bar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!bar_try(bar, parity))
+    if (clock64() - t0 > kWaitCycles) return false;
+  return true;
+}
+__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(bar, parity)); }
 
 __device__ __forceinline__ float p_ex2(float x) {
   float y;
@@ -53,34 +67,36 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __grid_constant__ CUtensorMap mapK,
+__global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __grid_constant__ CUtensorMap mapK,
                                                                        const __grid_constant__ CUtensorMap mapV, const SharedAttn p,
                                                                        const uint32_t row_tiles) {
   using SM = PreSmem<D>;
-  constexpr uint32_t kS = 0, kP = D == 64 ? 128 : 0, kO = D == 64 ? 192 : 128;  // columns of tensor memory
-  constexpr bool kAhead = D == 64;  // scores of the next tile beside the weights of this one
+  constexpr uint32_t kSP = 128, kO = 256;  // columns of tensor memory: a stream's scores and weights, its sums behind both streams' scores
   constexpr uint32_t kTypes = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
-  extern __shared__ unsigned char pre_raw[];
-  unsigned char* const sm = reinterpret_cast<unsigned char*>(((uintptr_t)pre_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char pre_raw[];
+  unsigned char* const sm = pre_raw;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + SM::kBarOff);
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SM::kSlots + 5);
-  const uint32_t full0 = s_u32(bars), empty0 = s_u32(bars + SM::kSlots), q_ready = s_u32(bars + 2 * SM::kSlots), s_ready = q_ready + 8,
-                 s_free = q_ready + 16, p_ready = q_ready + 24, pv_done = q_ready + 32;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SM::kSlots + 7);
+  const uint32_t full0 = s_u32(bars), empty0 = s_u32(bars + SM::kSlots), q_ready = s_u32(bars + 2 * SM::kSlots);
+  auto s_ready = [&](uint32_t st) { return q_ready + 8 + 8 * st; };
+  auto p_ready = [&](uint32_t st) { return q_ready + 24 + 8 * st; };
+  auto pv_done = [&](uint32_t st) { return q_ready + 40 + 8 * st; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (uint32_t i = 0; i < SM::kSlots; ++i) {
       bar_init(full0 + 8 * i, 1);
       bar_init(empty0 + 8 * i, 1);
     }
-    bar_init(q_ready, 8);
-    bar_init(s_ready, 1);
-    bar_init(s_free, 8);
-    bar_init(p_ready, 8);
-    bar_init(pv_done, 1);
+    bar_init(q_ready, 16);
+    for (uint32_t st = 0; st < 2; ++st) {
+      bar_init(s_ready(st), 1);
+      bar_init(p_ready(st), 8);
+      bar_init(pv_done(st), 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(256u) : "memory");
+  if (warp == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   fence_before();
@@ -90,138 +106,127 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
   pdl_launch_dependents();  // the own rows do not wait for the shared ones, only the join does
 
   // CTAs of the same keys are neighbours
-  const uint32_t G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % row_tiles, g = blockIdx.x / row_tiles % p.kvH,
-                 split = blockIdx.x / row_tiles / p.kvH;
-  const uint32_t row0 = tile * kPreRows, all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles,
-                 n = min(p.pre_tiles, all - first);  // tiles of keys
+  const bool twice = row_tiles == 1;  // one row tile: the streams have it both
+  const uint32_t pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
+                 split = blockIdx.x / pairs / p.kvH;
+  const uint32_t all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles, n = min(p.pre_tiles, all - first);  // tiles of keys
+  const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
   bool ok = true;
 
-  if (warp == 8) {
+  if (warp == 16) {
     uint32_t j = 0;
     auto load = [&](const CUtensorMap* map, uint32_t it) {
       const uint32_t s = j % SM::kSlots;
-      if (j >= SM::kSlots && !warp_wait(empty0 + 8 * s, (j / SM::kSlots - 1) & 1)) return ok = false;
+      if (j >= SM::kSlots && !all_wait_for(empty0 + 8 * s, (j / SM::kSlots - 1) & 1)) return ok = false;
       if (elect_one()) {
         bar_expect_tx(full0 + 8 * s, SM::kTile);
 #pragma unroll
         for (uint32_t b = 0; b < D / 64; ++b)
-          tma_load_2d(s_u32(sm) + SM::kQ + s * SM::kTile + b * (kPreTile * 128), map, (int)(g * D + b * 64), (int)((first + it) * kPreTile), full0 + 8 * s);
+          tma_load_2d(s_u32(sm) + SM::kRing + s * SM::kTile + b * (kPreTile * 128), map, (int)(g * D + b * 64), (int)((first + it) * kPreTile), full0 + 8 * s);
       }
       ++j;
       return true;
     };
-    if constexpr (kAhead) {
+    if (twice) {  // K0 K1, V0 K2, V1 K3, ..
       load(&mapK, 0);
-      for (uint32_t it = 0; it < n && ok; ++it) {
-        if (it + 1 < n && !load(&mapK, it + 1)) break;
-        if (!load(&mapV, it)) break;
-      }
-    } else {
+      if (n > 1 && ok) load(&mapK, 1);
+      for (uint32_t u = 0; u < n && ok; ++u)
+        if (!load(&mapV, u) || (u + 2 < n && !load(&mapK, u + 2))) break;
+    } else {  // K0 V0, K1 V1, ..
       for (uint32_t it = 0; it < n && ok; ++it)
         if (!load(&mapK, it) || !load(&mapV, it)) break;
     }
     if (ok) ok = drain_ring<SM::kSlots>(empty0, j);
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // 16-bit operands, float32 sums; A along K in both products; B along K (K tile) or along N (V tile)
     constexpr uint32_t idesc_s = kTypes | ((kPreTile >> 3) << 17) | ((kPreRows >> 4) << 24);
     constexpr uint32_t idesc_o = kTypes | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((kPreRows >> 4) << 24);
-    const uint32_t q_s = s_u32(sm);
-    uint32_t j = 0;
-    auto slot = [&](uint32_t& s) {  // wait for the next tile
-      s = j % SM::kSlots;
-      ok = warp_wait(full0 + 8 * s, (j / SM::kSlots) & 1);
-      fence_after();
-      ++j;
-      return ok;
-    };
-    auto scores = [&]() {
-      uint32_t s;
-      if (!slot(s)) return false;
+    const uint32_t base = s_u32(sm);
+    // the slot of the keys of unit u, and of its values
+    auto keys_of = [&](uint32_t u) { return twice ? (u < 2 ? u : 2 * u - 1) : (u >> 1) * 2; };
+    auto values_of = [&](uint32_t u) { return twice ? (u + 2 < units ? 2 * u + 2 : units + u) : (u >> 1) * 2 + 1; };
+    auto arrived = [&](uint32_t j) { return ok = all_wait_for(full0 + 8 * (j % SM::kSlots), (j / SM::kSlots) & 1); };
+    auto scores = [&](uint32_t u) {
+      const uint32_t st = u & 1, s = keys_of(u) % SM::kSlots;
       if (elect_one()) {
-        const uint32_t k_s = q_s + SM::kQ + s * SM::kTile;
+        const uint32_t k_s = base + SM::kRing + s * SM::kTile, q_s = base + st * SM::kQ;
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (kPreRows * 128) + (kk & 3) * 32;
-          umma_f16(tmem + kS, smem_desc_sw128(q_s + off), smem_desc_sw128(k_s + off), idesc_s, kk != 0);
+          umma_f16(tmem + st * kSP, smem_desc_sw128(q_s + off), smem_desc_sw128(k_s + off), idesc_s, kk != 0);
         }
-        umma_commit(empty0 + 8 * s);
-        umma_commit(s_ready);
+        if (twice || st) umma_commit(empty0 + 8 * s);
+        umma_commit(s_ready(st));  // (arrives when everything issued before is done, this stream's product before included)
       }
-      return true;
     };
-    ok = warp_wait(q_ready, 0);
-    fence_after();
-    if (ok) scores();
-    for (uint32_t it = 0; it < n && ok; ++it) {
-      if (kAhead && it + 1 < n) {
-        if (!(ok = warp_wait(s_free, it & 1))) break;
-        fence_after();
-        if (!scores()) break;
-      }
-      if (!(ok = warp_wait(p_ready, it & 1))) break;
+    ok = all_wait_for(q_ready, 0);
+    for (uint32_t u = 0; u < 2 && u < units && ok; ++u) {
+      if (!arrived(keys_of(u))) break;
       fence_after();
-      uint32_t s;
-      if (!slot(s)) break;
+      scores(u);
+    }
+    for (uint32_t u = 0; u < units && ok; ++u) {
+      const uint32_t st = u & 1, it = u >> 1, j = values_of(u);  // it: the stream's own count
+      const bool more = u + 2 < units;
+      // (the tiles first: the weights are what is waited for)
+      if (!arrived(j) || (more && !arrived(keys_of(u + 2)))) break;
+      if (!(ok = all_wait_for(p_ready(st), it & 1))) break;
+      fence_after();
       if (elect_one()) {
-        const uint32_t v_s = q_s + SM::kQ + s * SM::kTile;
+        const uint32_t s = j % SM::kSlots, v_s = base + SM::kRing + s * SM::kTile;
 #pragma unroll
         for (uint32_t kk = 0; kk < kPreTile / 16; ++kk)
-          umma_f16_ta(tmem + kO, tmem + kP + kk * 8, smem_desc_mn_sw128(v_s + kk * 2048, kPreTile * 128), idesc_o, (it | kk) != 0);
-        umma_commit(empty0 + 8 * s);
-        umma_commit(pv_done);
+          umma_f16_ta(tmem + kO + st * D, tmem + st * kSP + kk * 8, smem_desc_mn_sw128(v_s + kk * 2048, kPreTile * 128), idesc_o, (it | kk) != 0);
+        if (twice || st) umma_commit(empty0 + 8 * s);
+        if (!more) umma_commit(pv_done(st));
       }
       // (the weights lie where the next scores go: products of one thread run in their order)
-      if (!kAhead && it + 1 < n && !scores()) break;
+      if (more) scores(u + 2);
     }
   } else {
+    // Up to 64 rows twice: the second stream has them in the other half of the lanes, whose warps sit on other schedulers.
+    const uint32_t st = warp >> 3, row0 = (tile + (twice ? 0u : st)) * kPreRows - (twice && st && R <= 64 ? 64u : 0u);  // (below 0: no row)
     {  // the rows of Q as they are
       constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;
       const uint32_t c = (lane % kLanes) * 8;
       const T* const q = reinterpret_cast<const T*>(p.q);
 #pragma unroll
       for (uint32_t i = 0; i < 16; i += kRows) {
-        const uint32_t r = warp * 16 + i + lane / kLanes, row = row0 + r, b = row / G;
+        const uint32_t r = (warp & 7) * 16 + i + lane / kLanes, row = row0 + r, b = row / G;
         const uint4 v = row < R ? __ldg(reinterpret_cast<const uint4*>(q + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + c)) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(sm + (c >> 6) * (kPreRows * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(sm + st * SM::kQ + (c >> 6) * (kPreRows * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4)) = v;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(q_ready);
     }
-    const uint32_t quarter = warp & 3, half = warp >> 2, col0 = half * (kPreTile / 2), r_own = quarter * 32 + lane, row = row0 + r_own;
-    const uint32_t lanes = tmem + (quarter * 32u << 16);
-    const bool there = row0 + quarter * 32 < R;  // some row of this warp is: else its exponentials are left out
+    __syncwarp();
+    if (lane == 0) bar_arrive(q_ready);
+    const uint32_t quarter = warp & 3, half = warp >> 2 & 1, col0 = half * (kPreTile / 2), r_own = quarter * 32 + lane, row = row0 + r_own;
+    const uint32_t lanes = tmem + (quarter * 32u << 16), cS = st * kSP, cO = kO + st * D;
+    const uint32_t tiles = twice ? (n + 1 - st) / 2 : n;  // of this stream
+    const bool there = __any_sync(0xffffffffu, row < R);  // else this warp's exponentials are left out
     const float c = p.scale2, growth = kGrowth / c, floor = c > 1.f ? -1e38f / c : -1e38f;
     const uint64_t c2 = pair(c, c);
-    float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff);  // [2][kPreRows]
-    auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(quarter + 1) : "memory"); };
+    float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff) + st * 2 * kPreRows;  // [half][row]
+    auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(st * 4 + quarter + 1) : "memory"); };
     auto either = [&](bool mine) {  // a condition on a row of either warp
       uint32_t r;
       asm volatile(
           "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
           : "=r"(r)
-          : "r"(quarter + 1), "r"((uint32_t)mine)
+          : "r"(st * 4 + quarter + 1), "r"((uint32_t)mine)
           : "memory");
       return r != 0;
     };
-    auto value = [&](uint32_t j) {  // the product of tile j with its values is done
-      ok = __all_sync(0xffffffffu, ok && bar_wait(pv_done, Values::parity(j)));
-    };
     float m = 0.f, l = 0.f;  // m: of the scores as they are
-    for (uint32_t it = 0; it < n; ++it) {
-      ok = __all_sync(0xffffffffu, ok && bar_wait(s_ready, it & 1));  // (a warp that gave up still meets the other one)
-      if (!kAhead) Values::at_tile(it, value);
+    for (uint32_t it = 0; it < tiles; ++it) {
+      // these scores are there, and the product with the tile before's values is done (a warp that gave up still meets the other one)
+      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(st), it & 1));
       if (!there) {
-        if (kAhead) {
-          __syncwarp();
-          if (lane == 0) bar_arrive(s_free);
-          Values::at_tile(it, value);
-        }
         __syncwarp();
-        if (lane == 0) bar_arrive(p_ready);
+        if (lane == 0) bar_arrive(p_ready(st));
         continue;
       }
-      const uint32_t n0 = (first + it) * kPreTile + col0;
+      const uint32_t n0 = (first + (twice ? it * 2 + st : it)) * kPreTile + col0;
       // The weights are formed from the maximum as it stands; a row that turns out to have grown too far (the first tile always
       // has) makes its two warps raise their maxima and do the tile again.
       uint64_t sum[2];
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
       for (;;) {
         uint32_t s[kPreTile / 2];
         fence_after();
-        tmem_ld(lanes + kS + col0, s);
+        tmem_ld(lanes + cS + col0, s);
         if (n0 + kPreTile / 2 > p.prefix) {  // keys behind the last: nothing (their rows were filled with zeros)
 #pragma unroll
           for (uint32_t j = 0; j < kPreTile / 2; ++j)
@@ -247,17 +252,15 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
           meet();
           top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + r_own]), it ? m : floor);
           if (it) {
-            Values::at_rescaling(it, value);
-            fence_after();
             const float f = p_ex2((m - top) * c);
             l *= f;
 #pragma unroll 1
             for (uint32_t k = half * (D / 2); k < (half + 1) * (D / 2); k += 16) {
               uint32_t o[16];
-              tmem_ld(lanes + kO + k, o);
+              tmem_ld(lanes + cO + k, o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st(lanes + kO + k, o);
+              tmem_st(lanes + cO + k, o);
             }
           }
           m = top;
@@ -278,22 +281,15 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
           }
         };
         weights(0);
-        if (!kAhead) fence_before();  // (the other warp's scores may lie where this one's weights go: both have read theirs now)
+        fence_before();  // (the other warp's scores may lie where this one's weights go: both have read theirs now)
         if (either(top > m + growth) && !raise) {
           raise = true;
           continue;
         }
-        if (!kAhead) fence_after();
-        if (kAhead) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(s_free);
-          Values::at_tile(it, value);  // the weights of the tile before have been used
-          fence_after();
-        }
-        tmem_st(lanes + kP + col0 / 2, w[0]);
+        fence_after();
+        tmem_st(lanes + cS + col0 / 2, w[0]);
         weights(1);
-        tmem_st(lanes + kP + col0 / 2 + 16, w[1]);
+        tmem_st(lanes + cS + col0 / 2 + 16, w[1]);
         break;
       }
       float s0, s1;
@@ -302,14 +298,14 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
       tmem_st_wait();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(p_ready);
+      if (lane == 0) bar_arrive(p_ready(st));
     }
-    Values::at_end(n, value);
+    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), 0));
     if (there) {
       swap[half * kPreRows + r_own] = l;
       meet();
       l += swap[(half ^ 1) * kPreRows + r_own];
-      const uint64_t at = ((uint64_t)split * p.kvH + g) * R + row;
+      const uint64_t at = ((uint64_t)(twice ? split * 2 + st : split) * p.kvH + g) * R + row;
       if (row < R && half == 0) {
         // Every score -infinity (a row's sum has the 1 of its maximum otherwise): as if there were no keys. A wait that gave up: NaN.
         float2 ml = make_float2(m * c, l);
@@ -317,16 +313,28 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
         if (!ok) ml = make_float2(0.f, __uint_as_float(0x7fffffffu));
         *reinterpret_cast<float2*>(p.pre_ml + at * 2) = ml;
       }
-      if (ok) {
+      if (ok && tiles) {
+        // By way of shared memory, so that a warp stores whole lines: the first stream's go where Q was (all scores have been multiplied
+        // when its last product is done), the second's to the ring (everything has). Pieces of 16 bytes, eight by eight in an order that
+        // follows from the row: no bank twice.
+        constexpr uint32_t kPieces = D / 8, kBytes = 32 * kPieces * 16;  // of a row's half, and of a warp's
+        unsigned char* const mine = sm + (st ? SM::kRing : 0u) + (warp & 7) * kBytes;
         fence_after();
-        float* const out = p.pre_o + at * D;
-#pragma unroll 1
-        for (uint32_t k = half * (D / 2); k < (half + 1) * (D / 2); k += 32) {
-          uint32_t o[32];
-          tmem_ld(lanes + kO + k, o);
-          if (row >= R) continue;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(out + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (uint32_t k = 0; k < kPieces; k += 8) {
+          uint32_t o[32];
+          tmem_ld(lanes + cO + half * (D / 2) + k * 4, o);
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(mine + lane * (kPieces * 16) + (k + (e ^ (lane & 7))) * 16) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+        __syncwarp();
+        const uint32_t first_row = row - lane;
+#pragma unroll 4
+        for (uint32_t i = lane; i < 32 * kPieces; i += 32) {
+          const uint32_t r = i / kPieces, e = i % kPieces;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * (kPieces * 16) + (e ^ (r & 7)) * 16);
+          if (first_row + r < R) *reinterpret_cast<uint4*>(p.pre_o + (at - lane + r) * D + half * (D / 2) + e * 4) = v;
         }
       }
     }
@@ -339,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_shared_umma_kernel(const __g
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+  if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 template <typename T, int D>
@@ -349,7 +357,8 @@ cudaError_t launch_pre(cudaStream_t s, const SharedAttn& p) {
   if (!encode_tile_map16(&mapK, p.kp, p.prefix, width, kPreTile) || !encode_tile_map16(&mapV, p.vp, p.prefix, width, kPreTile)) return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(attn_shared_umma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PreSmem<D>::kTotal);
   if (e != cudaSuccess) return e;
-  const uint64_t row_tiles = ((uint64_t)p.B * (p.qH / p.kvH) + kPreRows - 1) / kPreRows, grid = row_tiles * p.kvH * p.pre_splits;
+  const uint64_t row_tiles = ((uint64_t)p.B * (p.qH / p.kvH) + kPreRows - 1) / kPreRows;
+  const uint64_t grid = (row_tiles + 1) / 2 * p.kvH * (row_tiles == 1 ? p.pre_splits / 2 : p.pre_splits);
   if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
   attn_shared_umma_kernel<T, D><<<(unsigned)grid, kThreads, PreSmem<D>::kTotal, s>>>(mapK, mapV, p, (uint32_t)row_tiles);
   return cudaGetLastError();

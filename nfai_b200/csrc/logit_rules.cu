@@ -37,6 +37,12 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
   const float* const x = p.logits + base;
   float* const y = p.out + base;
 
+  // What decides what else is read comes first, the logits right behind it: nothing of the row is waited for twice.
+  int32_t hist_len = p.history && p.history_len ? __ldg(p.history_len + row) : 0x7fffffff;
+  int32_t bias_lo = p.n_bias ? __ldg(p.bias_start + row) : 0, bias_hi = p.n_bias ? __ldg(p.bias_start + row + 1) : 0;
+  const int64_t mrow = p.n_masks ? (p.mask_rows ? (int64_t)__ldg(p.mask_rows + row) : (int64_t)row) : -1;
+  const float rep = p.repetition ? __ldg(p.repetition + row) : 1.f, freq = p.frequency ? __ldg(p.frequency + row) : 0.f,
+              pres = p.presence ? __ldg(p.presence + row) : 0.f;
   float v[QUADS][4];
 #pragma unroll
   for (int k = 0; k < QUADS; ++k) {
@@ -52,30 +58,41 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
   float early = 0.f;  // tokens in front of the first quad: the first slice's
   const bool has_early = slice == 0 && tid < peel;
   if (has_early) early = x[tid];
-
-  uint32_t n_hist = 0;
-  if (p.history) {
-    n_hist = p.history_stride;
-    if (p.history_len) n_hist = (uint32_t)min((int64_t)max(p.history_len[row], 0), (int64_t)p.history_stride);
+  const bool masked = mrow >= 0 && mrow < (int64_t)p.n_masks;
+  uint32_t allowed[QUADS], allowed_early = 0xffffffffu;
+  if (masked) {
+    const uint32_t* const mask = p.masks + (uint64_t)mrow * ((p.V + 31) / 32);
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) {
+      const uint32_t t = t0 + (k * kLT + tid) * 4;
+      allowed[k] = t < t1 ? __funnelshift_r(__ldg(mask + (t >> 5)), __ldg(mask + (min(t + 3, p.V - 1) >> 5)), t & 31) : 0u;
+    }
+    if (has_early) allowed_early = __ldg(mask) >> tid;
+  } else {
+#pragma unroll
+    for (int k = 0; k < QUADS; ++k) allowed[k] = 0xffffffffu;
   }
-  uint32_t b0 = 0, b1 = 0;
-  if (p.n_bias) {
-    b0 = (uint32_t)min(max(p.bias_start[row], 0), (int)min(p.n_bias, 0x7fffffffu));
-    b1 = (uint32_t)min(max(p.bias_start[row + 1], 0), (int)min(p.n_bias, 0x7fffffffu));
-  }
+  const uint32_t n_hist = p.history ? (uint32_t)min((int64_t)max(hist_len, 0), (int64_t)p.history_stride) : 0u;
+  const uint32_t b0 = min((uint32_t)max(bias_lo, 0), p.n_bias), b1 = min((uint32_t)max(bias_hi, 0), p.n_bias);
   const bool counted = n_hist > 0, biased = b1 > b0;
   // a token's place in the tables; anything else (another slice's, no token at all): kTable
   auto cell = [&](uint32_t t) { return t >= t0 ? (t < t1 ? t - t0 : kTable) : (slice == 0 && t < peel ? S + t : kTable); };
   if (counted || biased) {
-    for (uint32_t i = tid; i < kTable; i += kLT) {
-      if (counted) count[i] = 0;
-      if (biased) listing[i] = 0;
+    for (uint32_t i = tid; i < kTable / 4; i += kLT) {
+      if (counted) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
+      if (biased) reinterpret_cast<uint4*>(listing)[i] = make_uint4(0, 0, 0, 0);
     }
     __syncthreads();
     const uint32_t* const h = p.history + (uint64_t)row * p.history_stride;
-    for (uint32_t i = tid; i < n_hist; i += kLT) {
-      const uint32_t c = cell(__ldg(h + i));
-      if (c != kTable) atomicAdd(count + c, 1u);
+    for (uint32_t i = tid; i < n_hist; i += kLT * 8) {  // eight at a time on their way
+      uint32_t t[8];
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) t[k] = i + k * kLT < n_hist ? __ldg(h + i + k * kLT) : 0xffffffffu;
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t c = cell(t[k]);
+        if (c != kTable) atomicAdd(count + c, 1u);
+      }
     }
     for (uint32_t i = b0 + tid; i < b1; i += kLT) {
       const uint32_t c = cell(__ldg(p.bias_ids + i));
@@ -83,10 +100,6 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     }
     __syncthreads();
   }
-  const float rep = p.repetition ? p.repetition[row] : 1.f, freq = p.frequency ? p.frequency[row] : 0.f, pres = p.presence ? p.presence[row] : 0.f;
-  const int64_t mrow = p.n_masks ? (p.mask_rows ? (int64_t)p.mask_rows[row] : (int64_t)row) : -1;
-  const bool masked = mrow >= 0 && mrow < (int64_t)p.n_masks;
-  const uint32_t* const mask = p.masks + (masked ? (uint64_t)mrow * ((p.V + 31) / 32) : 0);
   auto ruled = [&](float a, uint32_t c, uint32_t listed) {
     if (c) {
       a = a > 0.f ? __fdiv_rn(a, rep) : a * rep;
@@ -107,13 +120,9 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
       v[k][2] = ruled(v[k][2], c.z, l.z);
       v[k][3] = ruled(v[k][3], c.w, l.w);
     }
-    if (masked) {
-      const uint32_t w0 = __ldg(mask + (t >> 5)), w1 = __ldg(mask + (min(t + 3, p.V - 1) >> 5));
-      const uint32_t bits = __funnelshift_r(w0, w1, t & 31);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(bits >> i & 1)) v[k][i] = -INFINITY;
-    }
+    for (int i = 0; i < 4; ++i)
+      if (!(allowed[k] >> i & 1)) v[k][i] = -INFINITY;
     if (VEC && t + 4 <= t1) {
       *reinterpret_cast<float4*>(y + t) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
     } else {
@@ -124,7 +133,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
   }
   if (has_early) {
     early = ruled(early, counted ? count[S + tid] : 0u, biased ? listing[S + tid] : 0u);
-    if (masked && !(__ldg(mask) >> tid & 1)) early = -INFINITY;
+    if (!(allowed_early & 1)) early = -INFINITY;
     y[tid] = early;
   }
 }

@@ -33,8 +33,13 @@ template <typename T>
 struct Vec8 {  // eight elements as they lie in memory
   uint4 w[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = ld_stream16(reinterpret_cast<const uint4*>(p) + i);
+    if constexpr (sizeof(T) == 4) {  // 32 bytes in one request: a whole sector per thread
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z), "=r"(w[1].w)
+                   : "l"(p));
+    } else {
+      w[0] = ld_stream16(p);
+    }
   }
   __device__ __forceinline__ void widen(float (&f)[8]) const {
     if constexpr (sizeof(T) == 4) {
@@ -47,8 +52,10 @@ struct Vec8 {  // eight elements as they lie in memory
   }
 };
 __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(__float_as_uint(f[0])), "r"(__float_as_uint(f[1])),
+               "r"(__float_as_uint(f[2])), "r"(__float_as_uint(f[3])), "r"(__float_as_uint(f[4])), "r"(__float_as_uint(f[5])),
+               "r"(__float_as_uint(f[6])), "r"(__float_as_uint(f[7]))
+               : "memory");
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(kRT) rope_rows_any_kernel(const RopeRows p) {
 template <typename XT, typename OT, bool HALVES>
 cudaError_t launch_layout(cudaStream_t s, const RopeRows& p) {
   const uintptr_t all = (uintptr_t)p.x | (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v;
-  const bool wide = (all & 15) == 0 && p.d % 8 == 0 && p.dims % (HALVES ? 16 : 8) == 0 && p.x_stride % 8 == 0 && p.dims / 2 <= kMaxTable;
+  const bool wide = (all & 31) == 0 && p.d % 8 == 0 && p.dims % (HALVES ? 16 : 8) == 0 && p.x_stride % 8 == 0 && p.dims / 2 <= kMaxTable;
   if (!wide) {
     const uint64_t total = (uint64_t)p.rows * (p.qH + 2 * p.kvH) * p.d, blocks = (total + kRT - 1) / kRT;
     rope_rows_any_kernel<XT, OT, HALVES><<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), kRT, 0, s>>>(p);
