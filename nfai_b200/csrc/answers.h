@@ -63,7 +63,7 @@ struct SharedAttn {
   float* own_o = nullptr;             // [own_splits][B * qH][d]
   float* own_ml = nullptr;            // [own_splits][B * qH][2]
   uint32_t pre_splits = 0, pre_tiles = 0;  // parts of the shared rows, tiles of keys per CTA; 0: they are walked like a sequence's own
-  uint32_t own_splits = 1;
+  uint32_t own_splits = 1, own_least = 64; // parts of a sequence's keys at most, and keys of a part at least
   bool joined = false;                // more than one partial result per row: they go to scratch and a last kernel joins them
   uint32_t* err = nullptr;            // device word of the context; may be null
 };
@@ -71,7 +71,7 @@ struct SharedAttn {
 struct SharedPlan {
   bool tensor = false;                // own rows on the warp-level tensor kernel (else CUDA cores)
   uint32_t rows = 8;                  // query heads per CTA there
-  uint32_t pre_splits = 0, pre_tiles = 0, own_splits = 1;
+  uint32_t pre_splits = 0, pre_tiles = 0, own_splits = 1, own_least = 64;
   bool joined = false;
   size_t pre_o = 0, pre_ml = 0, own_o = 0, own_ml = 0, total = 0;  // byte offsets
 };

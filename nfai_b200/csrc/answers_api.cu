@@ -160,7 +160,7 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   p.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)d)) * 1.4426950408889634);
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
   p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
-  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.joined = plan.joined; p.err = c->dev_err;
+  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined; p.err = c->dev_err;
   return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan));
 }
 

@@ -5,6 +5,7 @@
 // This file holds the plan of a call and the kernel on the CUDA cores, for any type and head size: a CTA has the query heads of one KV
 // head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
 // (a quarter of the head each, all query heads), then a thread has four of the output's dimensions and every n-th key.
+#include <stdlib.h>
 #include "attn_shared_common.cuh"
 
 namespace nfai {
@@ -160,13 +161,14 @@ cudaError_t launch_any(cudaStream_t s, const SharedAttn& p) {
   const uint32_t hgroups = (p.qH / p.kvH + NR - 1) / NR;
   return launch_pdl(attn_shared_any_kernel<T, NR>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kST), smem, s, p.pre_splits != 0, p, hgroups);
 }
-// The join of partial results, a row of the output (sequence, query head) per WARPS warps: lanes have the parts' maxima and sums, then four
-// dimensions each, with the parts' rows asked for eight at a time.
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(kST) attn_shared_join_kernel(const SharedAttn p) {
-  constexpr int kRows = kST / 32 / WARPS;
-  __shared__ float part_ml[kST / 32][2];
-  __shared__ __align__(16) float part_o[WARPS > 1 ? kST / 32 : 1][256];
+// The join of partial results, a row of the output (sequence, query head) per WARPS warps. A lane has four dimensions (UNITS times) of a
+// part; where LANES of them are a whole row, the warp has 32 / LANES parts at once. Eight parts are on their way at a time.
+constexpr int kJT = 128;
+template <typename T, int WARPS, int LANES, int UNITS>
+__global__ void __launch_bounds__(kJT) attn_shared_join_kernel(const SharedAttn p) {
+  constexpr int kRows = kJT / 32 / WARPS, kAtOnce = 32 / LANES;
+  constexpr uint32_t kStep = WARPS * kAtOnce;
+  __shared__ __align__(16) float part_o[WARPS > 1 ? kJT / 32 : 1][UNITS * 128];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WARPS, row = blockIdx.x * kRows + warp / WARPS, d = p.d;
   pdl_wait();
   const bool there = row < p.B * p.qH;
@@ -174,109 +176,109 @@ __global__ void __launch_bounds__(kST) attn_shared_join_kernel(const SharedAttn 
   const Walk walk = walk_of(p, b, 0);
   const bool busy = there && !walk.idle;
   const uint32_t own = busy ? walk.parts : 0, n = busy ? own + p.pre_splits : 0;
-  const uint64_t BQ = (uint64_t)p.B * p.qH, R = (uint64_t)p.B * G, pre0 = (uint64_t)g * R + (uint64_t)b * G + (h - g * G);
-  auto at = [&](uint32_t i, const float*& o, const float*& ml) {  // part i
-    const uint64_t r = i < own ? (uint64_t)i * BQ + row : (uint64_t)(i - own) * p.kvH * R + pre0;
-    o = (i < own ? p.own_o : p.pre_o) + r * d;
-    ml = (i < own ? p.own_ml : p.pre_ml) + r * 2;
-  };
-  const uint32_t mine = n > sub ? (n - sub + WARPS - 1) / WARPS : 0;  // parts sub, sub + WARPS, ..
+  const uint64_t BQ = (uint64_t)p.B * p.qH, R = (uint64_t)p.B * G, pre_step = p.kvH * R, pre0 = (uint64_t)g * R + (uint64_t)b * G + (h - g * G);
+  // rows of parts, as offsets: a sequence's own, then the shared ones'
+  auto own_row = [&](uint32_t i) { return (uint64_t)i * BQ + row; };
+  auto pre_row = [&](uint32_t i) { return (uint64_t)(i - own) * pre_step + pre0; };
+  const uint32_t slot = sub * kAtOnce + lane / LANES, e = lane % LANES * 4;  // parts slot, slot + kStep, ..
+  const bool wide = UNITS > 1 || e < d;
   float M = -INFINITY, L = 0.f;
-  float4 acc[2] = {};
-  for (uint32_t k0 = 0; k0 < mine; k0 += 32) {
-    const uint32_t cnt = min(32u, mine - k0);
+  float4 acc[UNITS] = {};
+  for (uint32_t k0 = 0; k0 < n; k0 += 32) {  // 32 parts' maxima and sums, the same in every warp of the row
+    const uint32_t cnt = min(32u, n - k0);
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < cnt) {
-      const float *o, *x;
-      at(sub + (k0 + lane) * WARPS, o, x);
-      ml = __ldcg(reinterpret_cast<const float2*>(x));
-    }
+    if (lane < cnt) ml = __ldcg(reinterpret_cast<const float2*>(k0 + lane < own ? p.own_ml + own_row(k0 + lane) * 2 : p.pre_ml + pre_row(k0 + lane) * 2));
     const float top = fmaxf(M, warp_max(ml.x)), ref = top == -INFINITY ? 0.f : top, before = exp2f(M - ref), f = exp2f(ml.x - ref);
     M = top;
     // (a part without weights: nothing of it counts, but a sum that is not a number does)
     L = L * before + warp_sum(f != 0.f || ml.y != ml.y ? f * ml.y : 0.f);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < UNITS; ++u) {
       acc[u].x *= before; acc[u].y *= before; acc[u].z *= before; acc[u].w *= before;
     }
-    for (uint32_t k = 0; k < cnt; k += 8) {
-      float4 v[8][2];
+#pragma unroll 1
+    for (uint32_t k = slot; k < cnt + slot; k += 8 * kStep) {  // (the same count for all lanes: k - slot)
+      float4 v[8][UNITS];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float *o, *x;
-        at(sub + (k0 + min(k + j, cnt - 1)) * WARPS, o, x);
+        const uint32_t i = k + j * kStep;
+        const float* const o = (k0 + i < own ? p.own_o + own_row(k0 + i) * d : p.pre_o + pre_row(k0 + i) * d) + e;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (u * 128 + lane * 4 < d) v[j][u] = __ldcg(reinterpret_cast<const float4*>(o + u * 128 + lane * 4));
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float w = __shfl_sync(0xffffffffu, f, min(k + j, 31u));
-        if (k + j < cnt && w != 0.f) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (u * 128 + lane * 4 < d) {
-              acc[u].x = fmaf(w, v[j][u].x, acc[u].x); acc[u].y = fmaf(w, v[j][u].y, acc[u].y);
-              acc[u].z = fmaf(w, v[j][u].z, acc[u].z); acc[u].w = fmaf(w, v[j][u].w, acc[u].w);
-            }
+        for (int u = 0; u < UNITS; ++u) {
+          v[j][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < cnt && (UNITS > 1 ? u * 128 + e < d : wide)) v[j][u] = __ldcg(reinterpret_cast<const float4*>(o + u * 128));
         }
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t i = k + j * kStep;
+        float w = __shfl_sync(0xffffffffu, f, i & 31);
+        w = i < cnt ? w : 0.f;
+        if (w != 0.f) {
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u) {
+            acc[u].x = fmaf(w, v[j][u].x, acc[u].x); acc[u].y = fmaf(w, v[j][u].y, acc[u].y);
+            acc[u].z = fmaf(w, v[j][u].z, acc[u].z); acc[u].w = fmaf(w, v[j][u].w, acc[u].w);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = LANES; o < 32; o <<= 1) {  // the parts that the warp had at once
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      acc[u].x += __shfl_xor_sync(0xffffffffu, acc[u].x, o);
+      acc[u].y += __shfl_xor_sync(0xffffffffu, acc[u].y, o);
+      acc[u].z += __shfl_xor_sync(0xffffffffu, acc[u].z, o);
+      acc[u].w += __shfl_xor_sync(0xffffffffu, acc[u].w, o);
     }
   }
   if constexpr (WARPS > 1) {
-    if (lane == 0) {
-      part_ml[warp][0] = M;
-      part_ml[warp][1] = L;
-    }
+    if (lane < LANES) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (u * 128 + lane * 4 < d) *reinterpret_cast<float4*>(&part_o[warp][u * 128 + lane * 4]) = acc[u];
+      for (int u = 0; u < UNITS; ++u) *reinterpret_cast<float4*>(&part_o[warp][u * 128 + e]) = acc[u];
+    }
     __syncthreads();
     if (sub != 0) return;
-    const float first = M;
-    for (int w = 1; w < WARPS; ++w) M = fmaxf(M, part_ml[warp + w][0]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float f = exp2f(first - ref);
-    L = f != 0.f || L != L ? f * L : 0.f;
+    for (int w = 1; w < WARPS; ++w) {  // (all of them to the same maximum)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      acc[u].x *= f; acc[u].y *= f; acc[u].z *= f; acc[u].w *= f;
-    }
-    for (int w = 1; w < WARPS; ++w) {
-      f = exp2f(part_ml[warp + w][0] - ref);
-      const float l = part_ml[warp + w][1];
-      if (f == 0.f && l == l) continue;
-      L = fmaf(f, l, L);
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (u * 128 + lane * 4 < d) {
-          const float4 v = *reinterpret_cast<const float4*>(&part_o[warp + w][u * 128 + lane * 4]);
-          acc[u].x = fmaf(f, v.x, acc[u].x); acc[u].y = fmaf(f, v.y, acc[u].y);
-          acc[u].z = fmaf(f, v.z, acc[u].z); acc[u].w = fmaf(f, v.w, acc[u].w);
-        }
+      for (int u = 0; u < UNITS; ++u) {
+        const float4 v = *reinterpret_cast<const float4*>(&part_o[warp + w][u * 128 + e]);
+        acc[u].x += v.x; acc[u].y += v.y; acc[u].z += v.z; acc[u].w += v.w;
+      }
     }
   }
-  if (!busy) return;
+  if (!busy || lane >= LANES) return;
   const float inv = p.prefix || walk.n ? 1.0f / L : 0.f;
   T* const out = reinterpret_cast<T*>(p.out) + (uint64_t)row * d;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const uint32_t e = u * 128 + lane * 4;
-    if (e < d) {
-      store_as(out + e, acc[u].x * inv);
-      store_as(out + e + 1, acc[u].y * inv);
-      store_as(out + e + 2, acc[u].z * inv);
-      store_as(out + e + 3, acc[u].w * inv);
+  for (int u = 0; u < UNITS; ++u) {
+    const uint32_t at = u * 128 + e;
+    if (at < d) {
+      alignas(16) T y[4];
+      store_as(y, acc[u].x * inv);
+      store_as(y + 1, acc[u].y * inv);
+      store_as(y + 2, acc[u].z * inv);
+      store_as(y + 3, acc[u].w * inv);
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + at) = *reinterpret_cast<const float4*>(y);
+      else *reinterpret_cast<uint2*>(out + at) = *reinterpret_cast<const uint2*>(y);
     }
   }
 }
 
+template <typename T, int LANES, int UNITS>
+cudaError_t launch_join_of(cudaStream_t s, const SharedAttn& p) {
+  const uint32_t rows = p.B * p.qH;
+  if (p.pre_splits + p.own_splits > 16 && rows < 148 * 32)
+    return launch_pdl(attn_shared_join_kernel<T, 4, LANES, UNITS>, dim3(rows), dim3(kJT), 0, s, true, p);
+  return launch_pdl(attn_shared_join_kernel<T, 1, LANES, UNITS>, dim3((rows + 3) / 4), dim3(kJT), 0, s, true, p);
+}
 template <typename T>
 cudaError_t launch_join(cudaStream_t s, const SharedAttn& p) {
-  const uint32_t rows = p.B * p.qH;
-  if (p.pre_splits + p.own_splits > 8 && rows < 148 * 64)
-    return launch_pdl(attn_shared_join_kernel<T, 4>, dim3((rows + 1) / 2), dim3(kST), 0, s, true, p);
-  return launch_pdl(attn_shared_join_kernel<T, 1>, dim3((rows + 7) / 8), dim3(kST), 0, s, true, p);
+  if (p.d == 32) return launch_join_of<T, 8, 1>(s, p);
+  if (p.d == 64) return launch_join_of<T, 16, 1>(s, p);
+  return p.d <= 128 ? launch_join_of<T, 32, 1>(s, p) : launch_join_of<T, 32, 2>(s, p);
 }
 
 template <typename T>
@@ -307,9 +309,10 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
   a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
-  // CTAs for every SM a few times over where the keys go so far (parts of 64 at least)
-  uint64_t parts = (148 * 4 + groups - 1) / groups;
-  if (parts > (keys + 63) / 64) parts = (keys + 63) / 64;
+  static const int kOver = getenv("XX_OVER") ? atoi(getenv("XX_OVER")) : 16, kMin = getenv("XX_MIN") ? atoi(getenv("XX_MIN")) : 64;
+  a.own_least = a.tensor ? kMin : 64;
+  uint64_t parts = (148 * (a.tensor ? kOver : 4) + groups - 1) / groups;
+  if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
   size_t off = 0;

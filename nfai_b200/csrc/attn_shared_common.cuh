@@ -8,6 +8,7 @@
 #include "answers.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "umma.cuh"
 
 namespace nfai {
 namespace shared_attn {
@@ -23,6 +24,18 @@ __device__ __forceinline__ float s_ex2(float x) {
   return y;
 }
 
+// Bounded waits as in umma.cuh; the limit is counted in cycles, whose counter is read in a few of them (the nanosecond timer takes
+// longer than some of these waits).
+constexpr long long kWaitCycles = 2000000000ll;
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+  if (umma::bar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!umma::bar_try(bar, parity))
+    if (clock64() - t0 > kWaitCycles) return false;
+  return true;
+}
+__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(bar, parity)); }
+
 // The walk of one CTA: keys [t0, t1) of sequence b's n, the shared rows first unless they have kernels of their own.
 struct Walk {
   uint32_t n, t0, t1, parts;  // parts: CTAs that this sequence's keys are divided among
@@ -34,7 +47,7 @@ __device__ __forceinline__ Walk walk_of(const SharedAttn& p, uint32_t b, uint32_
   w.idle = len < 0;
   const uint32_t own = w.idle ? 0u : min((uint32_t)len, p.capacity);
   w.n = own + (p.pre_splits ? 0u : p.prefix);
-  const uint32_t chunk = max(64u, ((w.n + p.own_splits - 1) / p.own_splits + 63) / 64 * 64);
+  const uint32_t chunk = max(p.own_least, ((w.n + p.own_splits - 1) / p.own_splits + 15) / 16 * 16);
   w.parts = max(1u, (w.n + chunk - 1) / chunk);
   w.t0 = min(w.n, split * chunk);
   w.t1 = min(w.n, w.t0 + chunk);

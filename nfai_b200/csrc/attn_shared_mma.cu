@@ -3,11 +3,12 @@
 //
 // Bound by HBM: a sequence's rows serve its own query heads only. The query heads of a KV head are the rows of a 16-row tile, both
 // products are mma.sync.m16n8k16 with float32 sums, the maximum and the sum of a row run along. A CTA of four warps has one KV head of
-// one sequence and a part of its keys, dealt to the warps 16 at a time; every warp is a pipeline of its own with 16-byte cp.async into
-// padded stages, so that nothing but a warp barrier stands between a copy and its use. What lies behind the last row is not read:
-// its place in a stage is filled with zeros and its score is -infinity.
-// A weight is split into two 16-bit terms (two products into one sum): the products wait for memory anyway, and nothing of the
-// weight is lost.
+// one sequence and a part of its keys, dealt to the warps in slices of 16. Every warp is a pipeline of its own that one lane feeds by
+// TMA (as 16-byte copies of all lanes the addresses took more issue slots than the products: 85 against 80 us with 64 sequences behind
+// 32768 rows); at the end the warps are joined in shared memory. Rows behind the last that counts may come with a slice: their scores
+// are -infinity and their values are overwritten with zeros. Warps that walk whole parts one after the other, asking for the next while
+// they multiply this one's last, spare the joining but not the wait for the warp with one part more: 77 us for 68 with 256 sequences. A weight is split into two 16-bit terms (two products into one sum): the products wait for memory anyway, and nothing of
+// the weight is lost.
 #include "attn_shared_common.cuh"
 
 namespace nfai {
@@ -15,18 +16,11 @@ namespace nfai {
 namespace {
 
 using namespace shared_attn;
+using namespace umma;
 
 constexpr int kMW = 4, kMT = kMW * 32;
 constexpr uint32_t kSlice = 16;  // keys per slice
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait_all_but() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a));
 }
@@ -69,50 +63,77 @@ struct Half<__nv_bfloat16> {
 
 template <int D>
 struct Shape {
-  static constexpr int kStages = D == 128 ? 3 : 4;
-  static constexpr int kLd = D + 8;  // elements of a staged row: 16 bytes more than it has, so that ldmatrix meets no bank twice
-  static constexpr int kHalf = kSlice * kLd;  // elements of a slice of K or V
-  static constexpr size_t kRing = (size_t)kMW * kStages * 2 * kHalf * 2;
+  static constexpr int kStages = 2;  // more of them leave room for fewer CTAs: 79 us with 2, 82 with 3, 93 with 4 (64 sequences behind 32768 rows)
+  static constexpr uint32_t kRowBytes = D == 32 ? 64 : 128;              // of a block: 32 or 64 elements, swizzled
+  static constexpr uint32_t kBlock = kSlice * kRowBytes;
+  static constexpr uint32_t kBlocks = D == 32 ? 1 : D / 64;
+  static constexpr uint32_t kHalf = kBlocks * kBlock;                    // a slice of K or V
+  static constexpr uint32_t kRing = kMW * kStages * 2 * kHalf;
+  static constexpr uint32_t kTotal = kRing + kMW * kStages * 8 + 1024;   // (blocks begin on 1024 bytes)
+  // piece c (16 bytes) of row r of a slice
+  static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
+    if constexpr (D == 32) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+    return (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  }
 };
+
 template <int D, int ROWS>
-constexpr size_t mma_smem() {
-  constexpr size_t merge = (size_t)(kMW + 1) * ROWS * (D + 4) * 4 + (kMW + 1) * ROWS * 2 * 4;
-  return Shape<D>::kRing > merge ? Shape<D>::kRing : merge;
+constexpr size_t mma_smem() {  // the stages, or what the warps are joined in
+  constexpr size_t join = ((size_t)(kMW + 1) * ROWS * (D + 4) + (kMW + 1) * ROWS * 2) * 4 + 1024;
+  return Shape<D>::kTotal > join ? Shape<D>::kTotal : join;
 }
 
 // ROWS: 8 or 16 query heads
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p, const uint32_t hgroups) {
+__global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_constant__ CUtensorMap pre_k, const __grid_constant__ CUtensorMap pre_v,
+                                                              const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
+                                                              const SharedAttn p, const uint32_t hgroups) {
   using SH = Shape<D>;
-  constexpr int NST = SH::kStages, LD = SH::kLd, HALF = SH::kHalf, R = ROWS / 8;
-  extern __shared__ __align__(16) unsigned char sm_mma[];
+  constexpr int NST = SH::kStages, R = ROWS / 8;
+  extern __shared__ unsigned char mma_raw[];
+  unsigned char* const sm = reinterpret_cast<unsigned char*>(((uintptr_t)mma_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, qr = lane >> 2, qc = (lane & 3) * 2, G = p.qH / p.kvH;
-  const uint32_t hg = blockIdx.x % hgroups, g = blockIdx.x / hgroups % p.kvH, b = blockIdx.x / hgroups / p.kvH;
-  const uint32_t h0 = g * G + hg * ROWS, nh = min((uint32_t)ROWS, G - hg * ROWS), split = blockIdx.y;
+  const uint32_t hg = blockIdx.x % hgroups, g = blockIdx.x / hgroups % p.kvH, b = blockIdx.x / hgroups / p.kvH, split = blockIdx.y;
+  const uint32_t h0 = g * G + hg * ROWS, nh = min((uint32_t)ROWS, G - hg * ROWS);
   const Walk walk = walk_of(p, b, split);
   if (walk.idle || split >= walk.parts) return leave(p);
-  const uint32_t slices = (walk.t1 - walk.t0 + kSlice - 1) / kSlice, mine = warp < slices ? (slices - warp + kMW - 1) / kMW : 0;
-  const uint32_t kvDim = p.kvH * D;
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm_mma) + warp * NST * 2 * HALF * 2;
-  constexpr uint32_t CPR = D / 8;  // 16-byte pieces of a row
-  const uint32_t c8 = (lane % CPR) * 8;
-  auto issue = [&](uint32_t i) {
-    const uint32_t n0 = walk.t0 + (i * kMW + warp) * kSlice, at = ring + (i % NST) * 2 * HALF * 2;
-#pragma unroll
-    for (uint32_t k = 0; k < kSlice * CPR / 32; ++k) {
-      const uint32_t r = lane / CPR + k * (32 / CPR), t = n0 + r;
-      const bool in = t < walk.t1;
-      bool own;
-      const uint64_t off = key_row(p, b, in ? t : walk.t0, own) * kvDim + g * D + c8;  // an address inside even where nothing is copied
-      cp16(at + (r * LD + c8) * 2, reinterpret_cast<const T*>(own ? p.ko : p.kp) + off, in ? 16u : 0u);
-      cp16(at + (HALF + r * LD + c8) * 2, reinterpret_cast<const T*>(own ? p.vo : p.vp) + off, in ? 16u : 0u);
-    }
-  };
-#pragma unroll
-  for (uint32_t i = 0; i < NST - 1; ++i) {
-    if (i < mine) issue(i);
-    cp_commit();  // (an empty group keeps the count uniform)
+  // slices of the shared rows first, then of the sequence's own: none has keys of both
+  const uint32_t shared = p.pre_splits ? 0u : p.prefix, cut = min(max(shared, walk.t0), walk.t1);
+  const uint32_t before = (cut - walk.t0 + kSlice - 1) / kSlice, slices = before + (walk.t1 - cut + kSlice - 1) / kSlice;
+  auto first_of = [&](uint32_t i) { return i < before ? walk.t0 + i * kSlice : cut + (i - before) * kSlice; };
+  auto count_of = [&](uint32_t i) { return min(kSlice, (i < before ? cut : walk.t1) - first_of(i)); };
+  unsigned char* const stages = sm + warp * NST * 2 * SH::kHalf;
+  const uint32_t ring = s_u32(stages), full = s_u32(sm + SH::kRing) + warp * NST * 8;
+  if (lane == 0) {
+    for (int i = 0; i < NST; ++i) bar_init(full + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncwarp();
+  uint32_t fill = 0;
+  auto issue = [&](uint32_t i) {
+    if (elect_one()) {
+      const uint32_t at = ring + fill * 2 * SH::kHalf, bar = full + 8 * fill, x = g * D, t = first_of(i);
+      const bool own = i >= before;
+      const CUtensorMap *const k = own ? &own_k : &pre_k, *const v = own ? &own_v : &pre_v;
+      const int row = (int)(own ? t - shared : t), seq = own ? (int)b : 0;
+      bar_expect_tx(bar, 2 * SH::kHalf);
+#pragma unroll
+      for (uint32_t j = 0; j < SH::kBlocks; ++j) {
+        tma_load_3d(at + j * SH::kBlock, k, (int)(x + j * 64), row, seq, bar);
+        tma_load_3d(at + SH::kHalf + j * SH::kBlock, v, (int)(x + j * 64), row, seq, bar);
+      }
+    }
+    fill = fill + 1 == NST ? 0 : fill + 1;
+  };
+#pragma unroll 1
+  for (uint32_t i = 0; i < NST - 1; ++i)
+    if (warp + i * kMW < slices) issue(warp + i * kMW);
+  // lanes of ldmatrix: keys of two position tiles (K), keys of a tile for two pieces of the head (V)
+  const uint32_t lm = lane >> 3, lr = lane & 7, k_row = (lm >> 1) * 8 + lr, v_row = (lm & 1) * 8 + lr;
+  bool ok = true;
+  uint32_t phase = 0;
+  uint32_t use = 0;
+
   // the queries as they are: the left operand, rows beyond the heads zero
   uint32_t q[D / 16][4];
   {
@@ -135,21 +156,26 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p
     m[r] = -INFINITY;
     l[r] = 0.f;
   }
-  const uint32_t lm = lane >> 3, lr = lane & 7;
-  const uint32_t k_lane = (((lm >> 1) * 8 + lr) * LD + (lm & 1) * 8) * 2, v_lane = (((lm & 1) * 8 + lr) * LD + (lm >> 1) * 8) * 2;
-
-  for (uint32_t i = 0; i < mine; ++i) {
+#pragma unroll 1
+  for (uint32_t i = warp; i < slices; i += kMW) {
+    const uint32_t cnt = count_of(i);
     __syncwarp();  // every lane is past its reads of the stage that is filled next
-    if (i + NST - 1 < mine) issue(i + NST - 1);
-    cp_commit();
-    cp_wait_all_but<NST - 1>();
-    __syncwarp();
-    const uint32_t n0 = walk.t0 + (i * kMW + warp) * kSlice, ks = ring + (i % NST) * 2 * HALF * 2, vs = ks + HALF * 2;
+    if (i + (NST - 1) * kMW < slices && ok) issue(i + (NST - 1) * kMW);
+    ok = __all_sync(0xffffffffu, ok && wait_for(full + 8 * use, phase));
+    const uint32_t ks = ring + use * 2 * SH::kHalf, vs = ks + SH::kHalf;
+    if (cnt < kSlice) {
+      unsigned char* const v = stages + (use * 2 + 1) * SH::kHalf;
+      for (uint32_t i = lane; i < (kSlice - cnt) * (D / 8); i += 32) *reinterpret_cast<uint4*>(v + SH::at(cnt + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (the stage's next copy comes behind these)
+      __syncwarp();
+    }
+    use = use + 1 == NST ? 0 : use + 1;
+    if (use == 0) phase ^= 1;
     float s[2][4] = {};
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       uint32_t b0, b1, b2, b3;
-      ldsm4(ks + kk * 32 + k_lane, b0, b1, b2, b3);
+      ldsm4(ks + SH::at(k_row, kk * 2 + (lm & 1)), b0, b1, b2, b3);
       Half<T>::mma(s[0], q[kk], b0, b1);
       Half<T>::mma(s[1], q[kk], b2, b3);
     }
@@ -157,10 +183,10 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float x[4] = {s[0][2 * r] * p.scale2, s[0][2 * r + 1] * p.scale2, s[1][2 * r] * p.scale2, s[1][2 * r + 1] * p.scale2};
-      if (n0 + kSlice > walk.t1) {
+      if (cnt < kSlice) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (n0 + (j >> 1) * 8 + qc + (j & 1) >= walk.t1) x[j] = -INFINITY;
+          if ((j >> 1) * 8 + qc + (j & 1) >= cnt) x[j] = -INFINITY;
       }
       float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -184,17 +210,22 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p
 #pragma unroll
     for (int j = 0; j < D / 8; j += 2) {
       uint32_t b0, b1, b2, b3;
-      ldsm4t(vs + j * 16 + v_lane, b0, b1, b2, b3);
+      ldsm4t(vs + SH::at(v_row, j + (lm >> 1)), b0, b1, b2, b3);
       Half<T>::mma(o[j], hi, b0, b1);
       Half<T>::mma(o[j + 1], hi, b2, b3);
       Half<T>::mma(o[j], lo, b0, b1);
       Half<T>::mma(o[j + 1], lo, b2, b3);
     }
   }
-  cp_wait_all_but<0>();
+  if (!ok) {
+    if (lane == 0 && p.err) atomicOr(p.err, 4u);
+    // copies may still be on their way: a bounded time for them to end before their memory is used for something else
+    for (volatile uint32_t spin = 0; spin < (1u << 20); ++spin) {
+    }
+  }
   __syncthreads();  // every warp is past its last read of its stages: the warps' rows go where they were
   constexpr uint32_t PL = D + 4;
-  float* const part = reinterpret_cast<float*>(sm_mma);            // [kMW][ROWS][PL]
+  float* const part = reinterpret_cast<float*>(sm);                // [kMW][ROWS][PL]
   float* const rows = part + kMW * ROWS * PL;                      // [ROWS][PL]
   float* const ml = rows + ROWS * PL;                              // [kMW][ROWS][2]
   float* const M = ml + kMW * ROWS * 2;                            // [ROWS], [ROWS]
@@ -203,30 +234,34 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const SharedAttn p
   for (int r = 0; r < R; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (!ok) l[r] = __uint_as_float(0x7fffffffu);
     const uint32_t row = qr + r * 8;
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(part + (warp * ROWS + row) * PL + j * 8 + qc) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-    if ((lane & 3) == 0) {
-      ml[(warp * ROWS + row) * 2] = m[r];
-      ml[(warp * ROWS + row) * 2 + 1] = l[r];
-    }
+    if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (warp * ROWS + row) * 2) = make_float2(m[r], l[r]);
   }
   __syncthreads();
-  for (uint32_t i = tid; i < nh * D; i += kMT) {
-    const uint32_t j = i / D, e = i % D;
+  for (uint32_t i = tid; i < nh * (D / 4); i += kMT) {
+    const uint32_t j = i / (D / 4), e = i % (D / 4) * 4;
+    float2 w[kMW];
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kMW; ++w) top = fmaxf(top, ml[(w * ROWS + j) * 2]);
-    float acc = 0.f, sum = 0.f;
+    for (int k = 0; k < kMW; ++k) {
+      w[k] = *reinterpret_cast<const float2*>(ml + (k * ROWS + j) * 2);
+      top = fmaxf(top, w[k].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMW; ++w) {
-      const float mw = ml[(w * ROWS + j) * 2], f = mw == -INFINITY ? 0.f : s_ex2(mw - top), lw = ml[(w * ROWS + j) * 2 + 1];
-      if (f != 0.f || lw != lw) {
-        acc = fmaf(f, part[(w * ROWS + j) * PL + e], acc);
-        sum = fmaf(f, lw, sum);
+    for (int k = 0; k < kMW; ++k) {
+      const float f = w[k].x == -INFINITY ? 0.f : s_ex2(w[k].x - top);
+      if (f != 0.f || w[k].y != w[k].y) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (k * ROWS + j) * PL + e);
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+        sum = fmaf(f, w[k].y, sum);
       }
     }
-    rows[j * PL + e] = acc;
+    *reinterpret_cast<float4*>(rows + j * PL + e) = acc;
     if (e == 0) {
       M[j] = top;
       L[j] = sum;
@@ -242,7 +277,15 @@ cudaError_t launch_rows(cudaStream_t s, const SharedAttn& p) {
   cudaError_t e = cudaFuncSetAttribute(attn_shared_mma_kernel<T, D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const uint32_t hgroups = (p.qH / p.kvH + ROWS - 1) / ROWS;
-  return launch_pdl(attn_shared_mma_kernel<T, D, ROWS>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kMT), smem, s, p.pre_splits != 0, p, hgroups);
+  CUtensorMap pre_k{}, pre_v{}, own_k{}, own_v{};
+  const uint64_t width = (uint64_t)p.kvH * D;
+  constexpr uint32_t kElems = D == 32 ? 32 : 64;
+  if (p.prefix && !p.pre_splits && (!encode_cache_map16(&pre_k, p.kp, 1, p.prefix, width, kElems, kSlice) || !encode_cache_map16(&pre_v, p.vp, 1, p.prefix, width, kElems, kSlice)))
+    return cudaErrorInvalidValue;
+  if (p.capacity && (!encode_cache_map16(&own_k, p.ko, p.B, p.capacity, width, kElems, kSlice) || !encode_cache_map16(&own_v, p.vo, p.B, p.capacity, width, kElems, kSlice)))
+    return cudaErrorInvalidValue;
+  return launch_pdl(attn_shared_mma_kernel<T, D, ROWS>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kMT), smem, s, p.pre_splits != 0, pre_k, pre_v,
+                    own_k, own_v, p, hgroups);
 }
 template <typename T, int D>
 cudaError_t launch_d(cudaStream_t s, const SharedAttn& p, uint32_t rows) {

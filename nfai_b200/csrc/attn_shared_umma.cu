@@ -15,7 +15,6 @@
 #include <type_traits>
 
 #include "attn_shared_common.cuh"
-#include "umma.cuh"
 
 namespace nfai {
 
@@ -24,6 +23,8 @@ namespace {
 using namespace umma;
 using shared_attn::kPreRows;
 using shared_attn::kPreTile;
+using shared_attn::all_wait_for;
+using shared_attn::wait_for;
 
 constexpr int kThreads = 576;
 constexpr float kGrowth = 8.0f;
@@ -39,18 +40,6 @@ struct PreSmem {
   static constexpr uint32_t kTotal = kSwapOff + 4 * kPreRows * 4;
 };
 static_assert(PreSmem<64>::kTotal <= 232448 && PreSmem<128>::kTotal <= 232448, "shared memory of a CTA");
-
-// Bounded waits as in umma.cuh; the limit is counted in cycles, whose counter is read in a few of them (the nanosecond timer takes
-// longer than some of these waits).
-constexpr long long kWaitCycles = 2000000000ll;
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
-  if (bar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!bar_try(bar, parity))
-    if (clock64() - t0 > kWaitCycles) return false;
-  return true;
-}
-__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(bar, parity)); }
 
 __device__ __forceinline__ float p_ex2(float x) {
   float y;
@@ -82,6 +71,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   auto p_ready = [&](uint32_t st) { return q_ready + 24 + 8 * st; };
   auto pv_done = [&](uint32_t st) { return q_ready + 40 + 8 * st; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // CTAs of the same keys are neighbours
+  const bool twice = row_tiles == 1;  // one row tile: the streams have it both
+  const uint32_t pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
+                 split = blockIdx.x / pairs / p.kvH;
+  const uint32_t all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles, n = min(p.pre_tiles, all - first);  // tiles of keys
+  const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
+  // Softmax warps ask for their rows of Q before anything else: behind the first tiles of all CTAs they would be 6 us on their way.
+  // Up to 64 rows twice: the second stream has them in the other half of the lanes, whose warps sit on other schedulers.
+  constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // lanes to a row
+  const uint32_t st = warp >> 3, row0 = (tile + (twice ? 0u : st)) * kPreRows - (twice && st && R <= 64 ? 64u : 0u);  // (below 0: no row)
+  const uint32_t qc = (lane % kLanes) * 8;
+  uint4 rows_q[16 / kRows];
+  if (warp < 16) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / kRows; ++i) {
+      const uint32_t row = row0 + (warp & 7) * 16 + i * kRows + lane / kLanes, b = row / G;
+      rows_q[i] = row < R ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + qc))
+                          : make_uint4(0, 0, 0, 0);
+    }
+  }
   if (tid == 0) {
     for (uint32_t i = 0; i < SM::kSlots; ++i) {
       bar_init(full0 + 8 * i, 1);
@@ -104,13 +113,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();  // the own rows do not wait for the shared ones, only the join does
-
-  // CTAs of the same keys are neighbours
-  const bool twice = row_tiles == 1;  // one row tile: the streams have it both
-  const uint32_t pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
-                 split = blockIdx.x / pairs / p.kvH;
-  const uint32_t all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles, n = min(p.pre_tiles, all - first);  // tiles of keys
-  const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
   bool ok = true;
 
   if (warp == 16) {
@@ -184,20 +186,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       if (more) scores(u + 2);
     }
   } else {
-    // Up to 64 rows twice: the second stream has them in the other half of the lanes, whose warps sit on other schedulers.
-    const uint32_t st = warp >> 3, row0 = (tile + (twice ? 0u : st)) * kPreRows - (twice && st && R <= 64 ? 64u : 0u);  // (below 0: no row)
-    {  // the rows of Q as they are
-      constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;
-      const uint32_t c = (lane % kLanes) * 8;
-      const T* const q = reinterpret_cast<const T*>(p.q);
+    // the rows of Q as they are
 #pragma unroll
-      for (uint32_t i = 0; i < 16; i += kRows) {
-        const uint32_t r = (warp & 7) * 16 + i + lane / kLanes, row = row0 + r, b = row / G;
-        const uint4 v = row < R ? __ldg(reinterpret_cast<const uint4*>(q + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + c)) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(sm + st * SM::kQ + (c >> 6) * (kPreRows * 128) + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (uint32_t i = 0; i < 16 / kRows; ++i) {
+      const uint32_t r = (warp & 7) * 16 + i * kRows + lane / kLanes;
+      *reinterpret_cast<uint4*>(sm + st * SM::kQ + (qc >> 6) * (kPreRows * 128) + r * 128 + ((((qc & 63) >> 3) ^ (r & 7)) << 4)) = rows_q[i];
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) bar_arrive(q_ready);
     const uint32_t quarter = warp & 3, half = warp >> 2 & 1, col0 = half * (kPreTile / 2), r_own = quarter * 32 + lane, row = row0 + r_own;
