@@ -43,6 +43,7 @@ struct LogitRules {
   const uint32_t* masks = nullptr;    // [n_masks][(V + 31) / 32]
   uint32_t n_masks = 0;
   const int32_t* mask_rows = nullptr; // [rows]; null: row r has mask r
+  uint32_t* err = nullptr;            // device word of the context; may be null
 };
 cudaError_t launch_logit_rules(cudaStream_t s, const LogitRules& p);
 

@@ -118,7 +118,7 @@ int nfai_op_logit_rules(nfai_ctx* c, const float* logits, uint32_t rows, uint32_
   p.history = history; p.history_stride = history ? history_stride : 0; p.history_len = history_len;
   p.repetition = repetition; p.frequency = frequency; p.presence = presence;
   p.bias_start = bias_start; p.bias_ids = bias_ids; p.bias = bias; p.n_bias = n_bias;
-  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows;
+  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->dev_err;
   return finish(c, stream, launch_logit_rules(stream_of(c, stream), p));
 }
 

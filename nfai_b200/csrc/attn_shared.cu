@@ -5,7 +5,6 @@
 // This file holds the plan of a call and the kernel on the CUDA cores, for any type and head size: a CTA has the query heads of one KV
 // head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
 // (a quarter of the head each, all query heads), then a thread has four of the output's dimensions and every n-th key.
-#include <stdlib.h>
 #include "attn_shared_common.cuh"
 
 namespace nfai {
@@ -309,9 +308,11 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
   a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
-  static const int kOver = getenv("XX_OVER") ? atoi(getenv("XX_OVER")) : 16, kMin = getenv("XX_MIN") ? atoi(getenv("XX_MIN")) : 64;
-  a.own_least = a.tensor ? kMin : 64;
-  uint64_t parts = (148 * (a.tensor ? kOver : 4) + groups - 1) / groups;
+  // CTAs for every SM twice over (the CUDA cores' four times) where the keys go so far. A part has 128 keys at least where the walk of the
+  // shared rows hides the time it takes (8 sequences behind 2011 rows: 11.4 us, 11.9 with 64, 12.3 with 32; 5 behind 100003: 46.3, 45.5,
+  // 44.6), 32 where it is all there is (2 sequences of 340 keys: 5.9 us, 6.2 with 64, 6.1 with 128).
+  a.own_least = !a.tensor ? 64 : shared ? 128 : 32;
+  uint64_t parts = (148 * (a.tensor ? 2 : 4) + groups - 1) / groups;
   if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
