@@ -300,10 +300,8 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
     uint64_t parts = 148 / groups;
     parts = parts < 1 ? 1 : parts > kMaxPreSplits ? kMaxPreSplits : parts;
     a.pre_tiles = (uint32_t)((tiles + parts - 1) / parts);
-    // (one row tile: each of the CTA's two walks leaves a part of its own, and has a tile at least)
-    if (twice && a.pre_tiles < 2) a.pre_tiles = 2;
+    if (twice && a.pre_tiles < 2) a.pre_tiles = 2;  // (a tile for each of the CTA's streams)
     a.pre_splits = (tiles + a.pre_tiles - 1) / a.pre_tiles;
-    if (twice) a.pre_splits *= 2;
   }
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
   a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
@@ -334,6 +332,8 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
 
 cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, const SharedPlan& plan) {
   cudaError_t e = cudaSuccess;
+  // Each kernel starts while the one before drains; only the join waits. (The own rows first, so that they are done when the walk of the
+  // shared rows has its SMs, which it wants whole: 45.6 us for 43.2 with 5 sequences behind 100003 rows, 77.4 for 74.7 with 64 behind 32768.)
   if (plan.pre_splits) {
     e = launch_attn_shared_umma(s, dtype, p);
     if (e != cudaSuccess) return e;

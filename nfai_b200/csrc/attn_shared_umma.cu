@@ -3,15 +3,21 @@
 // The query heads of a KV head and the sequences are one list of rows (row = sequence * G + head of the group). A CTA has two streams of
 // 128 rows each, one accumulator lane a row, and walks a part of the keys in tiles of 128. With more than 128 rows the streams are
 // neighbouring row tiles on the same keys, which are then fetched once for 256 rows; with fewer they are the same rows on every second
-// tile of keys, and leave two parts for the join. While one stream forms its weights the tensor pipe works for the other:
+// tile of keys. While one stream forms its weights the tensor pipe works for the other:
 //   warp 16  K and V tiles by TMA into a ring of 128-byte swizzled slots, in the order in which they are multiplied
 //   warp 17  one lane issues S(0), S(1), then for every unit (stream, tile) u: O += P(u) V, S(u + 2) = Q K^T, with P in tensor memory where S(u)
-//            was and V as it lies (its rows run along N)
+//            was and V as it lies (its rows run along N). (A warp for each stream was no faster, 76 us for 72 with 64 sequences behind 32768
+//            rows: the streams fell into step and wanted the same units at the same time.)
+//   warp 18  sees the ring's slots fill, in order, and arrives with the softmax warps on the barrier that warp 17 waits for: waiting for the
+//            tiles itself cost that warp 600 of 3700 cycles in which nothing was multiplied
 //   warps 0-7 and 8-15  softmax of a stream, two threads to a row (64 keys each): weights back into tensor memory as the 16-bit
-//            operand of the second product, their float32 sums kept; at the end (sums of weighted values, maximum, sum of weights) go
-//            to scratch, and attn_shared_join_kernel joins them with those of the own rows.
-// Warps whose rows are not there leave the exponentials out. Scores are products of the 16-bit queries as they are; the scale goes
-// into the exponent's multiply-add. A row's sums are rescaled only when its maximum has grown by more than 2^8 since the last time.
+//            operand of the second product, their float32 sums kept
+// Up to 64 (32) rows are in the lanes twice (four times), each copy with the weights of its own half (quarter) of a tile's keys and zeros
+// for the others: a row's exponentials are then spread over the schedulers, whose warps each see 32 lanes only.
+// At the end sums of weighted values, maxima and sums of weights go to scratch line by line, by way of shared memory, where streams and
+// copies of the same rows are joined; attn_shared_join_kernel joins the parts with those of the own rows.
+// Scores are products of the 16-bit queries as they are; the scale goes into the exponent's multiply-add. A row's sums are rescaled only
+// when its maximum has grown by more than 2^8 since the last time.
 #include <type_traits>
 
 #include "attn_shared_common.cuh"
@@ -21,12 +27,12 @@ namespace nfai {
 namespace {
 
 using namespace umma;
+using shared_attn::all_wait_for;
 using shared_attn::kPreRows;
 using shared_attn::kPreTile;
-using shared_attn::all_wait_for;
 using shared_attn::wait_for;
 
-constexpr int kThreads = 576;
+constexpr int kSoftmax = 512, kThreads = kSoftmax + 96;
 constexpr float kGrowth = 8.0f;
 
 template <int D>
@@ -36,10 +42,11 @@ struct PreSmem {
   static constexpr uint32_t kQ = kPreRows * D * 2;  // of one stream
   static constexpr uint32_t kRing = 2 * kQ;
   static constexpr uint32_t kBarOff = kRing + kSlots * kTile;
-  static constexpr uint32_t kSwapOff = kBarOff + 256;  // [stream][half][row]: maxima of the halves of a row, later their sums
+  static constexpr uint32_t kSwapOff = kBarOff + 256;  // [stream][half][row]: maxima of the halves of a row, later their sums, maxima and sums
   static constexpr uint32_t kTotal = kSwapOff + 4 * kPreRows * 4;
 };
 static_assert(PreSmem<64>::kTotal <= 232448 && PreSmem<128>::kTotal <= 232448, "shared memory of a CTA");
+static_assert(2 * kPreRows * 64 * 4 <= PreSmem<64>::kBarOff && 2 * kPreRows * 128 * 4 <= PreSmem<128>::kBarOff, "both streams' sums go where Q and the ring were");
 
 __device__ __forceinline__ float p_ex2(float x) {
   float y;
@@ -54,14 +61,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) {
+  __syncwarp();
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+using umma::tmem_st;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __grid_constant__ CUtensorMap mapK,
+// COPIES: how often the rows are in the lanes (2 and 4: one row tile)
+template <typename T, int D, int COPIES>
+__global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __grid_constant__ CUtensorMap mapQ,
+                                                                       const __grid_constant__ CUtensorMap mapK,
                                                                        const __grid_constant__ CUtensorMap mapV, const SharedAttn p,
                                                                        const uint32_t row_tiles) {
   using SM = PreSmem<D>;
   constexpr uint32_t kSP = 128, kO = 256;  // columns of tensor memory: a stream's scores and weights, its sums behind both streams' scores
   constexpr uint32_t kTypes = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
+  constexpr uint32_t kKeys = kPreTile / COPIES, kMine = kKeys / 2, kLanesOf = kPreRows / COPIES;  // of a copy: keys, a thread's keys, lanes
   extern __shared__ __align__(1024) unsigned char pre_raw[];
   unsigned char* const sm = pre_raw;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + SM::kBarOff);
@@ -72,35 +89,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   auto pv_done = [&](uint32_t st) { return q_ready + 40 + 8 * st; };
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // CTAs of the same keys are neighbours
-  const bool twice = row_tiles == 1;  // one row tile: the streams have it both
+  const bool twice = COPIES > 1 || row_tiles == 1;  // one row tile: the streams have it both
   const uint32_t pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
                  split = blockIdx.x / pairs / p.kvH;
   const uint32_t all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles, n = min(p.pre_tiles, all - first);  // tiles of keys
-  const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
-  // Softmax warps ask for their rows of Q before anything else: behind the first tiles of all CTAs they would be 6 us on their way.
-  // Up to 64 rows twice: the second stream has them in the other half of the lanes, whose warps sit on other schedulers.
-  constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // lanes to a row
-  const uint32_t st = warp >> 3, row0 = (tile + (twice ? 0u : st)) * kPreRows - (twice && st && R <= 64 ? 64u : 0u);  // (below 0: no row)
-  const uint32_t qc = (lane % kLanes) * 8;
-  uint4 rows_q[16 / kRows];
-  if (warp < 16) {
-#pragma unroll
-    for (uint32_t i = 0; i < 16 / kRows; ++i) {
-      const uint32_t row = row0 + (warp & 7) * 16 + i * kRows + lane / kLanes, b = row / G;
-      rows_q[i] = row < R ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + qc))
-                          : make_uint4(0, 0, 0, 0);
-    }
-  }
+  // Q comes by TMA where the rows of a copy are whole sequences' heads, by the softmax warps otherwise; one stream's, where both have the
+  // same. (By the softmax warps it holds up the first tiles by 1.6 us, or waits behind them for 6.)
+  const bool whole_q = kLanesOf % G == 0;
+  const uint32_t st = warp >> 3, row0 = (tile + (twice ? 0u : st)) * kPreRows;
   if (tid == 0) {
     for (uint32_t i = 0; i < SM::kSlots; ++i) {
       bar_init(full0 + 8 * i, 1);
       bar_init(empty0 + 8 * i, 1);
     }
-    bar_init(q_ready, 16);
-    for (uint32_t st = 0; st < 2; ++st) {
-      bar_init(s_ready(st), 1);
-      bar_init(p_ready(st), 8);
-      bar_init(pv_done(st), 1);
+    bar_init(q_ready, whole_q ? 2 : 17);
+    for (uint32_t i = 0; i < 2; ++i) {
+      bar_init(s_ready(i), 1);
+      bar_init(p_ready(i), 9);
+      bar_init(pv_done(i), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -113,9 +119,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents();  // the own rows do not wait for the shared ones, only the join does
+  const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
   bool ok = true;
 
   if (warp == 16) {
+    if (whole_q && elect_one()) {
+      const uint32_t streams = twice ? 1 : 2;
+      bar_expect_tx(q_ready, streams * SM::kQ);
+      for (uint32_t i = 0; i < streams; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < COPIES; ++k)
+#pragma unroll
+          for (uint32_t b = 0; b < D / 64; ++b)
+            tma_load_4d(s_u32(sm) + i * SM::kQ + b * (kPreRows * 128) + k * (kLanesOf * 128), &mapQ, (int)(b * 64), 0, (int)g, (int)((tile + i) * kPreRows / G), q_ready);
+    }
+    __syncwarp();
     uint32_t j = 0;
     auto load = [&](const CUtensorMap* map, uint32_t it) {
       const uint32_t s = j % SM::kSlots;
@@ -144,14 +162,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     constexpr uint32_t idesc_s = kTypes | ((kPreTile >> 3) << 17) | ((kPreRows >> 4) << 24);
     constexpr uint32_t idesc_o = kTypes | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((kPreRows >> 4) << 24);
     const uint32_t base = s_u32(sm);
-    // the slot of the keys of unit u, and of its values
+    // the place in the ring's order of the keys of unit u, and of its values
     auto keys_of = [&](uint32_t u) { return twice ? (u < 2 ? u : 2 * u - 1) : (u >> 1) * 2; };
     auto values_of = [&](uint32_t u) { return twice ? (u + 2 < units ? 2 * u + 2 : units + u) : (u >> 1) * 2 + 1; };
-    auto arrived = [&](uint32_t j) { return ok = all_wait_for(full0 + 8 * (j % SM::kSlots), (j / SM::kSlots) & 1); };
     auto scores = [&](uint32_t u) {
       const uint32_t st = u & 1, s = keys_of(u) % SM::kSlots;
       if (elect_one()) {
-        const uint32_t k_s = base + SM::kRing + s * SM::kTile, q_s = base + st * SM::kQ;
+        const uint32_t k_s = base + SM::kRing + s * SM::kTile, q_s = base + (twice ? 0u : st * SM::kQ);
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (kPreRows * 128) + (kk & 3) * 32;
@@ -161,18 +178,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         umma_commit(s_ready(st));  // (arrives when everything issued before is done, this stream's product before included)
       }
     };
-    ok = all_wait_for(q_ready, 0);
-    for (uint32_t u = 0; u < 2 && u < units && ok; ++u) {
-      if (!arrived(keys_of(u))) break;
-      fence_after();
-      scores(u);
-    }
+    ok = all_wait_for(q_ready, 0);  // Q, and the first keys' tiles
+    fence_after();
+    for (uint32_t u = 0; u < 2 && u < units && ok; ++u) scores(u);
     for (uint32_t u = 0; u < units && ok; ++u) {
       const uint32_t st = u & 1, it = u >> 1, j = values_of(u);  // it: the stream's own count
       const bool more = u + 2 < units;
-      // (the tiles first: the weights are what is waited for)
-      if (!arrived(j) || (more && !arrived(keys_of(u + 2)))) break;
-      if (!(ok = all_wait_for(p_ready(st), it & 1))) break;
+      if (!(ok = all_wait_for(p_ready(st), it & 1))) break;  // the weights, the values' tile and the next scores' keys
       fence_after();
       if (elect_one()) {
         const uint32_t s = j % SM::kSlots, v_s = base + SM::kRing + s * SM::kTile;
@@ -185,24 +197,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       // (the weights lie where the next scores go: products of one thread run in their order)
       if (more) scores(u + 2);
     }
-  } else {
-    // the rows of Q as they are
-#pragma unroll
-    for (uint32_t i = 0; i < 16 / kRows; ++i) {
-      const uint32_t r = (warp & 7) * 16 + i * kRows + lane / kLanes;
-      *reinterpret_cast<uint4*>(sm + st * SM::kQ + (qc >> 6) * (kPreRows * 128) + r * 128 + ((((qc & 63) >> 3) ^ (r & 7)) << 4)) = rows_q[i];
+  } else if (warp == 18) {
+    // All slots, each phase, in the ring's order: a wait knows a phase by its parity only.
+    const uint32_t tiles = 2 * n;
+    uint32_t seen = 0;
+    auto see = [&](uint32_t upto) {  // the first `upto` tiles have arrived
+      for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1);
+    };
+    see(min(tiles, twice ? 2u : 1u));
+    if (ok && lane == 0) bar_arrive(q_ready);
+    for (uint32_t u = 0; u < units && ok; ++u) {
+      const uint32_t st = u & 1, it = u >> 1;
+      see(min(tiles, twice ? 2 * u + 4 : (it + 1) * 2 + 1));
+      if (it && ok) ok = all_wait_for(p_ready(st), (it - 1) & 1);  // (the phase before has ended: this arrival is for the next)
+      if (ok && lane == 0) bar_arrive(p_ready(st));
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) bar_arrive(q_ready);
-    const uint32_t quarter = warp & 3, half = warp >> 2 & 1, col0 = half * (kPreTile / 2), r_own = quarter * 32 + lane, row = row0 + r_own;
+  } else {
+    if (!whole_q) {  // the rows as they are, each piece of 16 bytes to its place under the swizzle
+      constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // lanes to a row
+      const uint32_t qc = (lane % kLanes) * 8;
+      if (!twice || st == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i += kRows) {
+          const uint32_t r = (warp & 7) * 16 + i + lane / kLanes, row = row0 + r % kLanesOf, b = row / G;
+          const uint4 v = row < R ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + qc))
+                                  : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(sm + st * SM::kQ + (qc >> 6) * (kPreRows * 128) + r * 128 + ((((qc & 63) >> 3) ^ (r & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(q_ready);
+    }
+    const uint32_t quarter = warp & 3, half = warp >> 2 & 1, place = quarter * 32 + lane, copy = quarter / (4 / COPIES);
+    const uint32_t col0 = copy * kKeys + half * kMine, row = row0 + place % kLanesOf;
     const uint32_t lanes = tmem + (quarter * 32u << 16), cS = st * kSP, cO = kO + st * D;
     const uint32_t tiles = twice ? (n + 1 - st) / 2 : n;  // of this stream
     const bool there = __any_sync(0xffffffffu, row < R);  // else this warp's exponentials are left out
     const float c = p.scale2, growth = kGrowth / c, floor = c > 1.f ? -1e38f / c : -1e38f;
     const uint64_t c2 = pair(c, c);
-    float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff) + st * 2 * kPreRows;  // [half][row]
+    float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff) + st * 2 * kPreRows;  // [half][place]
     auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(st * 4 + quarter + 1) : "memory"); };
+    auto all_meet = [&]() { asm volatile("barrier.cta.sync 9, %0;" ::"n"(kSoftmax) : "memory"); };
     auto either = [&](bool mine) {  // a condition on a row of either warp
       uint32_t r;
       asm volatile(
@@ -226,26 +262,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       // has) makes its two warps raise their maxima and do the tile again.
       uint64_t sum[2];
       bool raise = it == 0;
+      constexpr uint32_t kPart = kMine < 32 ? kMine / 2 : 16;  // registers of packed weights that are stored at once
       for (;;) {
-        uint32_t s[kPreTile / 2];
+        uint32_t s[kMine];
         fence_after();
         tmem_ld(lanes + cS + col0, s);
-        if (n0 + kPreTile / 2 > p.prefix) {  // keys behind the last: nothing (their rows were filled with zeros)
+        if (n0 + kMine > p.prefix) {  // keys behind the last: nothing (their rows were filled with zeros)
 #pragma unroll
-          for (uint32_t j = 0; j < kPreTile / 2; ++j)
+          for (uint32_t j = 0; j < kMine; ++j)
             if (n0 + j >= p.prefix) s[j] = 0xff800000u;
         }
         float t[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
 #pragma unroll
-        for (uint32_t j = 4; j < kPreTile / 2; j += 8)
+        for (uint32_t j = 4; j < kMine; j += 8)
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i)
-            t[i] = j + 4 + i < kPreTile / 2 ? fmaxf(fmaxf(t[i], __uint_as_float(s[j + i])), __uint_as_float(s[j + 4 + i])) : fmaxf(t[i], __uint_as_float(s[j + i]));
+            t[i] = j + 4 + i < kMine ? fmaxf(fmaxf(t[i], __uint_as_float(s[j + i])), __uint_as_float(s[j + 4 + i])) : fmaxf(t[i], __uint_as_float(s[j + i]));
         float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         if (raise) {
-          swap[half * kPreRows + r_own] = top;
+          swap[half * kPreRows + place] = top;
           meet();
-          top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + r_own]), it ? m : floor);
+          top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + place]), it ? m : floor);
           if (it) {
             const float f = p_ex2((m - top) * c);
             l *= f;
@@ -262,29 +299,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         }
         sum[0] = sum[1] = 0;
         const uint64_t minus_m = pair(-m * c, -m * c);
-        uint32_t w[2][16];
-        auto weights = [&](uint32_t k) {
+        auto weights = [&](uint32_t k, uint32_t (&w)[kPart]) {
 #pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) {
-            const uint64_t x = fma2(pair(__uint_as_float(s[k * 32 + 2 * j]), __uint_as_float(s[k * 32 + 2 * j + 1])), c2, minus_m);
+          for (uint32_t j = 0; j < kPart; ++j) {
             float a, b;
-            unpair(x, a, b);
+            unpair(fma2(pair(__uint_as_float(s[(k * kPart + j) * 2]), __uint_as_float(s[(k * kPart + j) * 2 + 1])), c2, minus_m), a, b);
             a = p_ex2(a);
             b = p_ex2(b);
             sum[j & 1] = add2(sum[j & 1], pair(a, b));
-            w[k][j] = pack2(a, b, T());
+            w[j] = pack2(a, b, T());
           }
         };
-        weights(0);
+        uint32_t w[kPart];
+        weights(0, w);
         fence_before();  // (the other warp's scores may lie where this one's weights go: both have read theirs now)
         if (either(top > m + growth) && !raise) {
           raise = true;
           continue;
         }
         fence_after();
-        tmem_st(lanes + cS + col0 / 2, w[0]);
-        weights(1);
-        tmem_st(lanes + cS + col0 / 2 + 16, w[1]);
+        tmem_st(lanes + cS + col0 / 2, w);
+        if constexpr (COPIES == 1) {
+          uint32_t more[kPart];
+          weights(1, more);
+          tmem_st(lanes + cS + col0 / 2 + kPart, more);
+        } else {  // other copies' keys have no weight here
+          uint32_t zero[kPart] = {};
+#pragma unroll
+          for (uint32_t k = 1; k < COPIES; ++k) tmem_st(lanes + cS + (((copy + k) % COPIES) * kKeys + half * kMine) / 2, zero);
+        }
         break;
       }
       float s0, s1;
@@ -297,40 +340,69 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     }
     if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), 0));
     if (there) {
-      swap[half * kPreRows + r_own] = l;
+      swap[half * kPreRows + place] = l;
       meet();
-      l += swap[(half ^ 1) * kPreRows + r_own];
-      const uint64_t at = ((uint64_t)(twice ? split * 2 + st : split) * p.kvH + g) * R + row;
-      if (row < R && half == 0) {
-        // Every score -infinity (a row's sum has the 1 of its maximum otherwise): as if there were no keys. A wait that gave up: NaN.
-        float2 ml = make_float2(m * c, l);
-        if (l < 0.5f) ml = make_float2(-INFINITY, 0.f);
-        if (!ok) ml = make_float2(0.f, __uint_as_float(0x7fffffffu));
-        *reinterpret_cast<float2*>(p.pre_ml + at * 2) = ml;
+      l += swap[(half ^ 1) * kPreRows + place];
+    }
+    // Every score -infinity (a row's sum has the 1 of its maximum otherwise): as if there were no keys. A wait that gave up: NaN.
+    float2 ml = make_float2(m * c, l);
+    if (l < 0.5f) ml = make_float2(-INFINITY, 0.f);
+    if (!ok) ml = make_float2(0.f, __uint_as_float(0x7fffffffu));
+    // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
+    // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,
+    // eight by eight in an order that follows from the row: no bank is met twice.
+    if (twice) all_meet();
+    constexpr uint32_t kPieces = D / 4;
+    unsigned char* const sums = sm + st * (kPreRows * D * 4);
+    auto piece = [&](uint32_t at, uint32_t e) { return (at * kPieces + (e ^ (at & 7))) * 16; };
+    if (there && tiles && ok) {
+      fence_after();
+#pragma unroll
+      for (uint32_t k = 0; k < kPieces / 2; k += 8) {
+        uint32_t o[32];
+        tmem_ld(lanes + cO + half * (D / 2) + k * 4, o);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(sums + piece(place, half * (kPieces / 2) + k + e)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
       }
-      if (ok && tiles) {
-        // By way of shared memory, so that a warp stores whole lines: the first stream's go where Q was (all scores have been multiplied
-        // when its last product is done), the second's to the ring (everything has). Pieces of 16 bytes, eight by eight in an order that
-        // follows from the row: no bank twice.
-        constexpr uint32_t kPieces = D / 8, kBytes = 32 * kPieces * 16;  // of a row's half, and of a warp's
-        unsigned char* const mine = sm + (st ? SM::kRing : 0u) + (warp & 7) * kBytes;
-        fence_after();
+    }
+    if (twice) {
+      if (half == 0) {
+        swap[place] = ml.x;
+        swap[kPreRows + place] = ml.y;
+      }
+      all_meet();
+      const float* const mls = reinterpret_cast<const float*>(sm + SM::kSwapOff);
+      for (uint32_t i = tid; i < R * kPieces; i += kSoftmax) {  // a row's streams and copies
+        const uint32_t r = i / kPieces, e = i % kPieces;
+        float top = -INFINITY, f[2 * COPIES], total = 0.f;
+        auto from = [&](uint32_t k) { return (k / COPIES) * 2 * kPreRows + (k % COPIES) * kLanesOf + r; };
 #pragma unroll
-        for (uint32_t k = 0; k < kPieces; k += 8) {
-          uint32_t o[32];
-          tmem_ld(lanes + cO + half * (D / 2) + k * 4, o);
+        for (uint32_t k = 0; k < 2 * COPIES; ++k) top = fmaxf(top, f[k] = mls[from(k)]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (uint32_t e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(mine + lane * (kPieces * 16) + (k + (e ^ (lane & 7))) * 16) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        for (uint32_t k = 0; k < 2 * COPIES; ++k) {
+          f[k] = f[k] == -INFINITY ? 0.f : p_ex2(f[k] - top);
+          const float lk = mls[from(k) + kPreRows];
+          if (f[k] != 0.f || lk != lk) {
+            const float4 v = *reinterpret_cast<const float4*>(sm + (k / COPIES) * (kPreRows * D * 4) + piece((k % COPIES) * kLanesOf + r, e));
+            acc.x = fmaf(f[k], v.x, acc.x); acc.y = fmaf(f[k], v.y, acc.y); acc.z = fmaf(f[k], v.z, acc.z); acc.w = fmaf(f[k], v.w, acc.w);
+            total = fmaf(f[k], lk, total);
+          }
         }
-        __syncwarp();
-        const uint32_t first_row = row - lane;
+        const uint64_t at = ((uint64_t)split * p.kvH + g) * R + r;
+        *reinterpret_cast<float4*>(p.pre_o + at * D + e * 4) = acc;
+        if (e == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(top, total);
+      }
+    } else if (there) {
+      __syncwarp();
+      const uint64_t at0 = ((uint64_t)split * p.kvH + g) * R;
+      if (half == 0 && row < R) *reinterpret_cast<float2*>(p.pre_ml + (at0 + row) * 2) = ml;
 #pragma unroll 4
-        for (uint32_t i = lane; i < 32 * kPieces; i += 32) {
-          const uint32_t r = i / kPieces, e = i % kPieces;
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * (kPieces * 16) + (e ^ (r & 7)) * 16);
-          if (first_row + r < R) *reinterpret_cast<uint4*>(p.pre_o + (at - lane + r) * D + half * (D / 2) + e * 4) = v;
-        }
+      for (uint32_t i = lane; i < 32 * (kPieces / 2); i += 32) {
+        const uint32_t r = i / (kPieces / 2), e = half * (kPieces / 2) + i % (kPieces / 2);
+        const uint4 v = *reinterpret_cast<const uint4*>(sums + piece(quarter * 32 + r, e));
+        if (row - lane + r < R) *reinterpret_cast<uint4*>(p.pre_o + (at0 + row - lane + r) * D + e * 4) = v;
       }
     }
   }
@@ -345,18 +417,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-template <typename T, int D>
-cudaError_t launch_pre(cudaStream_t s, const SharedAttn& p) {
-  CUtensorMap mapK, mapV;
+template <typename T, int D, int COPIES>
+cudaError_t launch_copies(cudaStream_t s, const SharedAttn& p) {
+  CUtensorMap mapQ{}, mapK, mapV;
   const uint64_t width = (uint64_t)p.kvH * D;
   if (!encode_tile_map16(&mapK, p.kp, p.prefix, width, kPreTile) || !encode_tile_map16(&mapV, p.vp, p.prefix, width, kPreTile)) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(attn_shared_umma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PreSmem<D>::kTotal);
+  const uint32_t G = p.qH / p.kvH;
+  if (kPreRows / COPIES % G == 0 && !encode_query_map16(&mapQ, p.q, p.B, p.kvH, G, D, kPreRows / COPIES / G)) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(attn_shared_umma_kernel<T, D, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PreSmem<D>::kTotal);
   if (e != cudaSuccess) return e;
   const uint64_t row_tiles = ((uint64_t)p.B * (p.qH / p.kvH) + kPreRows - 1) / kPreRows;
-  const uint64_t grid = (row_tiles + 1) / 2 * p.kvH * (row_tiles == 1 ? p.pre_splits / 2 : p.pre_splits);
+  const uint64_t grid = (row_tiles + 1) / 2 * p.kvH * p.pre_splits;
   if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
-  attn_shared_umma_kernel<T, D><<<(unsigned)grid, kThreads, PreSmem<D>::kTotal, s>>>(mapK, mapV, p, (uint32_t)row_tiles);
+  attn_shared_umma_kernel<T, D, COPIES><<<(unsigned)grid, kThreads, PreSmem<D>::kTotal, s>>>(mapQ, mapK, mapV, p, (uint32_t)row_tiles);
   return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_pre(cudaStream_t s, const SharedAttn& p) {
+  const uint32_t rows = p.B * (p.qH / p.kvH);
+  return rows <= 32 ? launch_copies<T, D, 4>(s, p) : rows <= 64 ? launch_copies<T, D, 2>(s, p) : launch_copies<T, D, 1>(s, p);
 }
 
 }  // namespace

@@ -766,6 +766,17 @@ bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint6
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_query_map16(CUtensorMap* map, const void* base, uint64_t B, uint64_t kvH, uint64_t G, uint64_t D, uint32_t seqs) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || D % 64 || G > 256 || seqs > 256) return false;
+  cuuint64_t dims[4] = {D, G, kvH, B};
+  cuuint64_t strides[3] = {D * 2, G * D * 2, kvH * G * D * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)G, 1, seqs};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_stack_map16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t layers, uint64_t stride, uint32_t box_rows,
                         uint32_t box_blocks) {
   EncodeTiledFn fn = encode_fn();

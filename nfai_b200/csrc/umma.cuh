@@ -16,6 +16,9 @@ bool encode_stack_map16(CUtensorMap* map, const void* base, uint64_t rows, uint6
 // Tensor map of `seqs` caches of [rows][K] 16-bit elements one behind the other: box = box_elems elements (64, 128-byte swizzle, or 32,
 // 64-byte swizzle) x box_rows rows of one of them; zero fill outside. Coordinates: element, row, cache.
 bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint64_t rows, uint64_t K, uint32_t box_elems, uint32_t box_rows);
+// Tensor map of queries [B][kvH][G][D], 16-bit: box = 64 elements of the G heads of a KV head of `seqs` sequences, 128-byte swizzle, zero
+// fill outside. Coordinates: element, 0, KV head, sequence.
+bool encode_query_map16(CUtensorMap* map, const void* base, uint64_t B, uint64_t kvH, uint64_t G, uint64_t D, uint32_t seqs);
 // encode_tile_map16, kept for the next call with the same arguments: for operands that come again.
 bool tile_map16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows);
 
@@ -90,6 +93,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
 
