@@ -70,6 +70,7 @@ struct SharedAttn {
 };
 // What the sizes alone decide: which kernels run, into how many parts, and what scratch they need.
 struct SharedPlan {
+  uint32_t pre_warps = 0;             // shared rows on the CUDA cores: warps of a CTA (0: on tcgen05)
   bool tensor = false;                // own rows on the warp-level tensor kernel (else CUDA cores)
   uint32_t rows = 8;                  // query heads per CTA there
   uint32_t pre_splits = 0, pre_tiles = 0, own_splits = 1, own_least = 64;
@@ -79,6 +80,8 @@ struct SharedPlan {
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity);
 // the shared rows, partial results into pre_o and pre_ml; and everything else on the warp-level products
 cudaError_t launch_attn_shared_umma(cudaStream_t s, int dtype, const SharedAttn& p);
+cudaError_t launch_attn_shared_rows(cudaStream_t s, const SharedAttn& p, uint32_t warps);  // float32, eight queries a warp
+uint32_t attn_shared_rows_keys(uint32_t d);                                                // keys of its tiles
 cudaError_t launch_attn_shared_mma(cudaStream_t s, int dtype, const SharedAttn& p, uint32_t rows);
 cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, const SharedPlan& plan);
 

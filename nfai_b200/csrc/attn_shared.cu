@@ -15,7 +15,6 @@ using namespace shared_attn;
 
 constexpr int kST = 256;
 constexpr uint32_t kTK = 64;  // keys per tile
-constexpr uint32_t kSharedWalk = 512;  // shared rows from which on they are walked once for all
 
 __host__ __device__ constexpr uint32_t k_stride(uint32_t d) { return (d + 31) / 32 * 32 + 16; }  // two rows of a quarter-warp: other banks
 size_t any_smem_floats(uint32_t d, uint32_t rows) {
@@ -291,16 +290,27 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   SharedPlan a;
   const uint32_t G = qH / kvH;
   a.tensor = dtype != 0 && (d == 32 || d == 64 || d == 128);
-  const bool shared = dtype != 0 && (d == 64 || d == 128) && B >= 2 && prefix >= kSharedWalk;
+  const uint64_t R = (uint64_t)B * G;  // rows of a KV head
+  // The walk of the shared rows pays from a length on that makes up for its own two kernels. Measured, without | with it, 16-bit on either
+  // side of the rule: 64 sequences of 8 KV heads of 64 behind 430 rows, 16 behind 900, 4 behind 2500 take the same. float32: 16 sequences of
+  // 2 KV heads of 32 behind 1024 rows 12.0 | 10.1 us, 512: 8.4 | 9.8; 2 of 8 of 64 behind 2048: 15.4 | 12.2, 512: 8.5 | 10.0. One sequence
+  // gains from it in float32 only, whose other kernel keeps fewer loads on their way (8 KV heads of 128 behind 16384 rows 75.8 | 65.5, 4096:
+  // 27.2 | 28.8); in 16 bits that one is at the memory's rate (36000 rows: 82 us of 81).
+  const uint64_t work = (uint64_t)prefix * B * kvH * d;
+  const bool shared = dtype != 0 ? B >= 2 && (d == 64 || d == 128) && (uint64_t)prefix >= 200 + 6000000 / ((uint64_t)B * kvH * d) : work >= (B == 1 ? 4000000 : 1200000);
   if (shared) {
-    // one CTA on every SM, each with two tiles of 128 rows (sequence, head of the group), or one tile twice, and as many keys as the others
-    const uint32_t row_tiles = (uint32_t)(((uint64_t)B * G + kPreRows - 1) / kPreRows), twice = row_tiles == 1;
-    const uint64_t groups = (uint64_t)(row_tiles + 1) / 2 * kvH;
-    const uint32_t tiles = (prefix + kPreTile - 1) / kPreTile;
-    uint64_t parts = 148 / groups;
+    const bool umma = dtype != 0;
+    a.pre_warps = umma ? 0 : R <= 16 ? 2 : R <= 32 || d > 64 ? 4 : 8;
+    // On tcgen05 one CTA on every SM, each with two tiles of 128 rows (sequence, head of the group), or one tile twice; on the CUDA cores
+    // 16 warps, of 8 rows each, an SM. (36 rows in 5 warps of one CTA rather than 8: 48 us for 39; of heads of 128, 4 warps or 8: 33 | 38.)
+    // As many keys for one as for the others.
+    const uint64_t row_tiles = umma ? (R + kPreRows - 1) / kPreRows : (R + a.pre_warps * 8 - 1) / (a.pre_warps * 8);
+    const uint64_t groups = (umma ? (row_tiles + 1) / 2 : row_tiles) * kvH, room = umma ? 148 : 148 * 16 / a.pre_warps;
+    const uint32_t tile = umma ? kPreTile : attn_shared_rows_keys(d), tiles = (prefix + tile - 1) / tile;
+    uint64_t parts = room / groups;
     parts = parts < 1 ? 1 : parts > kMaxPreSplits ? kMaxPreSplits : parts;
     a.pre_tiles = (uint32_t)((tiles + parts - 1) / parts);
-    if (twice && a.pre_tiles < 2) a.pre_tiles = 2;  // (a tile for each of the CTA's streams)
+    if (umma && row_tiles == 1 && a.pre_tiles < 2) a.pre_tiles = 2;  // (a tile for each of the CTA's streams)
     a.pre_splits = (tiles + a.pre_tiles - 1) / a.pre_tiles;
   }
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
@@ -335,7 +345,7 @@ cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, c
   // Each kernel starts while the one before drains; only the join waits. (The own rows first, so that they are done when the walk of the
   // shared rows has its SMs, which it wants whole: 45.6 us for 43.2 with 5 sequences behind 100003 rows, 77.4 for 74.7 with 64 behind 32768.)
   if (plan.pre_splits) {
-    e = launch_attn_shared_umma(s, dtype, p);
+    e = plan.pre_warps ? launch_attn_shared_rows(s, p, plan.pre_warps) : launch_attn_shared_umma(s, dtype, p);
     if (e != cudaSuccess) return e;
   }
   if (plan.tensor) e = launch_attn_shared_mma(s, dtype, p, plan.rows);

@@ -201,7 +201,10 @@ ATTN_SIZES = [  # B, qH, kvH, d, P, cap, lens
     (2, 24, 8, 128, 2011, 1100, [1100, 1]), (9, 32, 8, 64, 2500, 64, [64, 0, -1, 5, 6, 7, 8, 9, 10]), (2, 3, 3, 8, 50, 20, [20, 0]),
     (2, 6, 2, 40, 90, 100, [100, 3]), (3, 10, 1, 80, 77, 10, [9, 0, 4]), (2, 4, 1, 256, 200, 90, [90, 0]), (1, 20, 1, 96, 70, 5, [5]),
     (40, 32, 8, 128, 1111, 20, [1 + b % 20 for b in range(40)]), (70, 32, 8, 64, 1300, 9, [b % 10 - 1 for b in range(70)]),
-    (33, 16, 1, 128, 640, 100, [3 * b for b in range(33)]), (2, 32, 8, 64, 9000, 16, [16, 2]), (1, 8, 8, 128, 5000, 3000, [2900])]
+    (33, 16, 1, 128, 640, 100, [3 * b for b in range(33)]), (2, 32, 8, 64, 9000, 16, [16, 2]), (1, 8, 8, 128, 5000, 3000, [2900]),
+    (20, 10, 5, 80, 600, 10, [b % 11 for b in range(20)]), (18, 4, 2, 256, 531, 4, [b % 5 - 1 for b in range(18)]), (17, 3, 3, 8, 777, 3, [b % 4 for b in range(17)]),
+    (70, 8, 8, 40, 513, 2, [b % 3 for b in range(70)]), (13, 20, 4, 64, 1000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 900, 5, [5, 4, 3, -1, 1, 0]),
+    (200, 8, 8, 40, 1513, 2, [b % 3 for b in range(200)]), (13, 20, 4, 64, 8000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 3900, 5, [5, 4, 3, -1, 1, 0])]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
