@@ -403,7 +403,8 @@ int nfai_op_sample_top_p(nfai_ctx* c, const float* logits, uint32_t V, float tem
  * `stream`: NULL runs on the context's own stream and returns when the result is there, as every nfai_op_* above. Otherwise it is a
  * cudaStream_t of the context's device (cudaStreamLegacy, the value 1, names the default stream): the work is put on that stream, the
  * call returns at once and may be captured into a graph; scratch and buffers must then not be used by work that may run at the same
- * time. The caller's current device stays what it was. */
+ * time. The caller's current device stays what it was. Kernels that wait for copies or products give up after a while, leave NaN in
+ * what they were to write, and note it: the next call without a stream to the attention or the rules returns NFAI_ERR_TIMEOUT then. */
 
 enum { NFAI_ROPE_PAIRS = 0 /* elements 2i and 2i+1, the reference's layout */, NFAI_ROPE_HALVES = 1 /* i and i + dims/2 */ };
 enum { NFAI_ROPE_PLAIN = 0, NFAI_ROPE_LINEAR = 1, NFAI_ROPE_BANDS = 2, NFAI_ROPE_YARN = 3 };
@@ -439,8 +440,7 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
  * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
  * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. What the rows behind
  * lens[b] hold makes no difference. scratch (device memory, 256-byte aligned) is used until the work is done;
- * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused).
- * Where a wait inside the tensor-core kernel gives up, the rows become NaN, and a call without a stream returns NFAI_ERR_TIMEOUT. */
+ * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused). */
 int nfai_op_attn_shared(nfai_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,
                         const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,
                         uint32_t d, float scale, void* out, void* scratch, size_t scratch_bytes, void* stream);

@@ -24,12 +24,18 @@ struct OnDevice {
 };
 
 // `stream` null: the context's stream, and the result is there on return; else the work is put on that stream.
+// waits: the kernels have waits that may give up, which they note in the context's word (calls on a stream before this one, too).
 cudaStream_t stream_of(nfai_ctx* c, void* stream) { return stream ? static_cast<cudaStream_t>(stream) : c->stream; }
-int finish(nfai_ctx* c, void* stream, cudaError_t launched) {
+int finish(nfai_ctx* c, void* stream, cudaError_t launched, bool waits) {
   if (launched != cudaSuccess)
     return fail(c, launched == cudaErrorInvalidValue ? NFAI_ERR_ARG : NFAI_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(launched));
-  if (!stream) CU(c, cudaStreamSynchronize(c->stream));
-  return NFAI_OK;
+  if (stream) return NFAI_OK;
+  uint32_t err = 0;
+  if (waits) CU(c, cudaMemcpyAsync(&err, c->dev_err, 4, cudaMemcpyDeviceToHost, c->stream));
+  CU(c, cudaStreamSynchronize(c->stream));
+  if (!err) return NFAI_OK;
+  CU(c, cudaMemsetAsync(c->dev_err, 0, 4, c->stream));
+  return fail(c, NFAI_ERR_TIMEOUT, "a bounded device-side wait gave up");
 }
 bool known_dtype(int t) { return t == NFAI_F32 || t == NFAI_F16 || t == NFAI_BF16; }
 #define ON_DEVICE(c)                                        \
@@ -94,7 +100,7 @@ int nfai_op_rope_rows(nfai_ctx* c, const void* x, int x_dtype, uint64_t x_stride
   p.x = x; p.x_stride = x_stride ? x_stride : width; p.rows = rows; p.qH = qH; p.kvH = kvH; p.d = d; p.dims = dims;
   p.halves = layout == NFAI_ROPE_HALVES; p.freqs = freqs; p.magnitude = magnitude; p.positions = positions; p.slots = slots;
   p.cache_rows = cache_rows; p.q = q_out; p.k = k_cache; p.v = v_cache;
-  return finish(c, stream, launch_rope_rows(stream_of(c, stream), x_dtype, out_dtype, p));
+  return finish(c, stream, launch_rope_rows(stream_of(c, stream), x_dtype, out_dtype, p), false);
 }
 
 int nfai_op_logit_rules(nfai_ctx* c, const float* logits, uint32_t rows, uint32_t V, const uint32_t* history, uint32_t history_stride,
@@ -119,7 +125,7 @@ int nfai_op_logit_rules(nfai_ctx* c, const float* logits, uint32_t rows, uint32_
   p.repetition = repetition; p.frequency = frequency; p.presence = presence;
   p.bias_start = bias_start; p.bias_ids = bias_ids; p.bias = bias; p.n_bias = n_bias;
   p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->dev_err;
-  return finish(c, stream, launch_logit_rules(stream_of(c, stream), p));
+  return finish(c, stream, launch_logit_rules(stream_of(c, stream), p), true);
 }
 
 // What is wrong with the sizes of an attention call; null: nothing.
@@ -161,7 +167,7 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
   p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
   p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined; p.err = c->dev_err;
-  return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan));
+  return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan), true);
 }
 
 }  // extern "C"

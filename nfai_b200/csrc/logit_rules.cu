@@ -129,9 +129,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     if (t < len) atomicAdd(count + t, 1u);
   }
   if (front && peel) in_front([&](uint32_t c, uint32_t) { atomicAdd(count + c, 1u); });
-  bool ok = true;
-  if (whole) ok = shared_attn::wait_for(bar, 0);
-  __syncthreads();  // the slice is there, and everything is counted
+  const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0));  // the slice is there, and everything is counted
   if (masked) {
 #pragma unroll
     for (uint32_t k = 0; k < kQuads; ++k) {
@@ -186,7 +184,14 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
       }
     }
   }
-  if (!ok && p.err && tid == 0) atomicOr(p.err, 4u);
+  if (!ok) {
+    if (p.err && tid == 0) atomicOr(p.err, 4u);
+    // the copy may still be on its way: a bounded time for it to end before its memory is used for something else
+    for (volatile uint32_t spin = 0; spin < (1u << 20); ++spin) {
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < whole; i += kLT) value[i] = __int_as_float(0x7fffffff);
+  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
   if (tid == 0 && whole) {
