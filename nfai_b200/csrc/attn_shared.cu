@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p
     q[i] = a;  // (the queries have been used)
   }
   __syncthreads();
-  leave_rows<T, kST>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l);
+  leave_rows<T, kST, false>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l, nullptr);
 }
 
 template <typename T, int NR>
@@ -331,7 +331,11 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
     return at;
   };
   const uint64_t rows = (uint64_t)B * qH;
-  a.joined = a.pre_splits || a.own_splits > 1;
+  // The kernel for the own rows adds the parts of the shared ones to its sums where a CTA has all of a sequence's keys and heads enough to
+  // make up for the wait, without a join | with one: 256 sequences of 32 over 8 heads of 64 behind 1500 rows 55.7 | 61.7 us, 128 behind 8000
+  // 49.2 | 52.6, 100 of 128 behind 4000 42.6 | 47.7, 64 of 128 behind 16000 (16 parts) 57.7 | 57.7, behind 32768 (18) 72.0 | 68.4; with one
+  // head a KV head, 300 of 16 of 64 behind 1500, 52.7 | 44.9. On the CUDA cores it takes registers that the walk needs: 10.8 us for 8.4.
+  a.joined = a.own_splits > 1 || (a.pre_splits && (!a.tensor || G < 4 || a.pre_splits > kFewParts));
   a.pre_ml = take(a.pre_splits * rows * 8);
   a.own_ml = take(a.joined ? a.own_splits * rows * 8 : 0);
   a.pre_o = take(a.pre_splits * rows * d * 4);

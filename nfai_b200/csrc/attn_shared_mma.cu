@@ -80,6 +80,7 @@ struct Shape {
 template <int D, int ROWS>
 constexpr size_t mma_smem() {  // the stages, or what the warps are joined in
   constexpr size_t join = ((size_t)(kMW + 1) * ROWS * (D + 4) + (kMW + 1) * ROWS * 2) * 4 + 1024;
+  static_assert(leave_room(ROWS, kMT) <= kMW * ROWS * (D + 4), "room");
   return Shape<D>::kTotal > join ? Shape<D>::kTotal : join;
 }
 
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
     }
   }
   __syncthreads();
-  leave_rows<T, kMT>(p, b, h0, nh, walk, split, rows, PL, M, L);
+  leave_rows<T, kMT, true>(p, b, h0, nh, walk, split, rows, PL, M, L, part);  // (the warps' rows have been used)
 }
 
 template <typename T, int D, int ROWS>

@@ -204,7 +204,9 @@ ATTN_SIZES = [  # B, qH, kvH, d, P, cap, lens
     (33, 16, 1, 128, 640, 100, [3 * b for b in range(33)]), (2, 32, 8, 64, 9000, 16, [16, 2]), (1, 8, 8, 128, 5000, 3000, [2900]),
     (20, 10, 5, 80, 600, 10, [b % 11 for b in range(20)]), (18, 4, 2, 256, 531, 4, [b % 5 - 1 for b in range(18)]), (17, 3, 3, 8, 777, 3, [b % 4 for b in range(17)]),
     (70, 8, 8, 40, 513, 2, [b % 3 for b in range(70)]), (13, 20, 4, 64, 1000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 900, 5, [5, 4, 3, -1, 1, 0]),
-    (200, 8, 8, 40, 1513, 2, [b % 3 for b in range(200)]), (13, 20, 4, 64, 8000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 3900, 5, [5, 4, 3, -1, 1, 0])]
+    (200, 8, 8, 40, 1513, 2, [b % 3 for b in range(200)]), (13, 20, 4, 64, 8000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 3900, 5, [5, 4, 3, -1, 1, 0]),
+    (33, 16, 1, 128, 2000, 100, [3 * b for b in range(33)]), (80, 20, 4, 64, 1900, 130, [b * 2 % 131 for b in range(80)]), (50, 32, 8, 64, 640, 17, [-1] * 49 + [3]),
+    (90, 24, 4, 128, 2100, 100, [b + 11 for b in range(90)])]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
@@ -230,11 +232,11 @@ def test_attention_peaked_scaled_and_repeated(cuda_ctx, kind, B, d, P):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("B,d,P", [(3, 64, 200), (24, 64, 1500), (24, 128, 1500), (3, 32, 300)])
-def test_attention_values_that_are_not_finite(cuda_ctx, kind, B, d, P):
+@pytest.mark.parametrize("B,d,P,G", [(3, 64, 200, 2), (24, 64, 1500, 2), (24, 128, 1500, 2), (3, 32, 300, 2), (80, 64, 1500, 4), (80, 128, 1500, 8)])
+def test_attention_values_that_are_not_finite(cuda_ctx, kind, B, d, P, G):
     """Keys that are -infinity towards a query have no weight; a row with no others is not a number; neither is one that sees a NaN; and
     other rows are as they were."""
-    s = attn_args(kind, B, 4, 2, d, P, 60, [b % 61 for b in range(B)], seed=3)
+    s = attn_args(kind, B, 2 * G, 2, d, P, 60, [b % 61 for b in range(B)], seed=3)
     s["q"] = s["q"].abs() + 0.5
     clean = dict(s, out=s["out"].clone())
     attn_call(cuda_ctx, clean)
@@ -246,16 +248,16 @@ def test_attention_values_that_are_not_finite(cuda_ctx, kind, B, d, P):
     # and sequence 1 has a NaN among its own values
     s["vo"].view(B, 60, 2, d)[1, 0, 0, 3] = math.nan
     attn_call(cuda_ctx, s)
-    out = s["out"].view(B, 2, 2, d)
+    out = s["out"].view(B, 2, G, d)
     assert out[:, 1].isnan().all()
     assert out[1, 0, :, 3].isnan().all() and out[1, 0, :, [0, 1, 2, 4]].isfinite().all()
     half = dict(clean, P=P // 2, kp=clean["kp"][:P // 2].contiguous(), vp=clean["vp"][:P // 2].contiguous(), out=s["out"].clone())
-    half["out"].view(B, 2, 2, d)[:, 1] = 0
+    half["out"].view(B, 2, G, d)[:, 1] = 0
     got = half["out"]
-    ref = attn_args(kind, B, 4, 2, d, P // 2, 60, [b % 61 for b in range(B)], seed=3)
+    ref = attn_args(kind, B, 2 * G, 2, d, P // 2, 60, [b % 61 for b in range(B)], seed=3)
     ref.update(q=clean["q"], kp=half["kp"], vp=half["vp"], ko=clean["ko"], vo=clean["vo"])
     attn_call(cuda_ctx, ref)
-    a, b = got.view(B, 2, 2, d)[2:, 0].double(), ref["out"].view(B, 2, 2, d)[2:, 0].double()
+    a, b = got.view(B, 2, G, d)[2:, 0].double(), ref["out"].view(B, 2, G, d)[2:, 0].double()
     assert (a - b).abs().max() <= 8 * half_step(TYPES[kind][0]) * b.abs().max() + 1e-5
 
 
