@@ -2,7 +2,7 @@
 // and over the sequence's own. Reference arithmetic: AttentionScoreCalculationShader.cs:170-205, AttentionSoftmaxShader.cs:145-177,
 // AttentionWeightedValueSumShader.cs:181-215, once per sequence.
 //
-// This file holds the plan of a call and the kernel on the CUDA cores, for any type and head size: a CTA has the query heads of one KV
+// This file holds the plan of a call, the join and the kernel on the CUDA cores, which serves float32 and heads above 128: a CTA has the query heads of one KV
 // head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
 // (a quarter of the head each, all query heads), then a thread has four of the output's dimensions and every n-th key.
 #include "attn_shared_common.cuh"
@@ -289,15 +289,16 @@ cudaError_t launch_own(cudaStream_t s, const SharedAttn& p, const SharedPlan& pl
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
   SharedPlan a;
   const uint32_t G = qH / kvH;
-  a.tensor = dtype != 0 && (d == 32 || d == 64 || d == 128);
+  a.tensor = dtype != 0 && d <= 128;
   const uint64_t R = (uint64_t)B * G;  // rows of a KV head
   // The walk of the shared rows pays from a length on that makes up for its own two kernels. Measured, without | with it, 16-bit on either
-  // side of the rule: 64 sequences of 8 KV heads of 64 behind 430 rows, 16 behind 900, 4 behind 2500 take the same. float32: 16 sequences of
+  // side of the rule: 64 sequences of 8 KV heads of 64 behind 430 rows, 16 behind 900, 4 behind 2500 take the same, 32 of 2 of 32 behind
+  // 2200, 250 behind 500. float32: 16 sequences of
   // 2 KV heads of 32 behind 1024 rows 12.0 | 10.1 us, 512: 8.4 | 9.8; 2 of 8 of 64 behind 2048: 15.4 | 12.2, 512: 8.5 | 10.0. One sequence
   // gains from it in float32 only, whose other kernel keeps fewer loads on their way (8 KV heads of 128 behind 16384 rows 75.8 | 65.5, 4096:
   // 27.2 | 28.8); in 16 bits that one is at the memory's rate (36000 rows: 82 us of 81).
   const uint64_t work = (uint64_t)prefix * B * kvH * d;
-  const bool shared = dtype != 0 ? B >= 2 && (d == 64 || d == 128) && (uint64_t)prefix >= 200 + 6000000 / ((uint64_t)B * kvH * d) : work >= (B == 1 ? 4000000 : 1200000);
+  const bool shared = dtype != 0 ? B >= 2 && d <= 128 && (uint64_t)prefix >= 200 + 6000000 / ((uint64_t)B * kvH * d) : work >= (B == 1 ? 4000000 : 1200000);
   if (shared) {
     const bool umma = dtype != 0;
     a.pre_warps = umma ? 0 : R <= 16 ? 2 : R <= 32 || d > 64 ? 4 : 8;

@@ -1,5 +1,5 @@
-// The own rows of every sequence (and the shared ones where they are few) on warp-level tensor products: 16-bit types, heads of 32, 64
-// and 128.
+// The own rows of every sequence (and the shared ones where they are few) on warp-level tensor products: 16-bit types, heads up to 128
+// (those that are not 32, 64 or 128 are filled up with zeros to the next of them by the copies).
 //
 // Bound by HBM: a sequence's rows serve its own query heads only. The query heads of a KV head are the rows of a 16-row tile, both
 // products are mma.sync.m16n8k16 with float32 sums, the maximum and the sum of a row run along. A CTA of four warps has one KV head of
@@ -113,15 +113,15 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
   uint32_t fill = 0;
   auto issue = [&](uint32_t i) {
     if (elect_one()) {
-      const uint32_t at = ring + fill * 2 * SH::kHalf, bar = full + 8 * fill, x = g * D, t = first_of(i);
+      const uint32_t at = ring + fill * 2 * SH::kHalf, bar = full + 8 * fill, t = first_of(i);
       const bool own = i >= before;
       const CUtensorMap *const k = own ? &own_k : &pre_k, *const v = own ? &own_v : &pre_v;
       const int row = (int)(own ? t - shared : t), seq = own ? (int)b : 0;
       bar_expect_tx(bar, 2 * SH::kHalf);
 #pragma unroll
       for (uint32_t j = 0; j < SH::kBlocks; ++j) {
-        tma_load_3d(at + j * SH::kBlock, k, (int)(x + j * 64), row, seq, bar);
-        tma_load_3d(at + SH::kHalf + j * SH::kBlock, v, (int)(x + j * 64), row, seq, bar);
+        tma_load_4d(at + j * SH::kBlock, k, (int)(j * 64), (int)g, row, seq, bar);
+        tma_load_4d(at + SH::kHalf + j * SH::kBlock, v, (int)(j * 64), (int)g, row, seq, bar);
       }
     }
     fill = fill + 1 == NST ? 0 : fill + 1;
@@ -138,13 +138,13 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
   // the queries as they are: the left operand, rows beyond the heads zero
   uint32_t q[D / 16][4];
   {
-    const T* const at = reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + h0) * D + qc;
+    const T* const at = reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + h0) * p.d + qc;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const uint32_t row = qr + (u & 1) * 8;
-        q[kk][u] = (u & 1) < R && row < nh ? __ldg(reinterpret_cast<const uint32_t*>(at + row * D + kk * 16 + (u >> 1) * 8)) : 0u;
+        const uint32_t row = qr + (u & 1) * 8, e = kk * 16 + (u >> 1) * 8;
+        q[kk][u] = (u & 1) < R && row < nh && e < p.d ? __ldg(reinterpret_cast<const uint32_t*>(at + row * p.d + e)) : 0u;
       }
     }
   }
@@ -279,11 +279,10 @@ cudaError_t launch_rows(cudaStream_t s, const SharedAttn& p) {
   if (e != cudaSuccess) return e;
   const uint32_t hgroups = (p.qH / p.kvH + ROWS - 1) / ROWS;
   CUtensorMap pre_k{}, pre_v{}, own_k{}, own_v{};
-  const uint64_t width = (uint64_t)p.kvH * D;
   constexpr uint32_t kElems = D == 32 ? 32 : 64;
-  if (p.prefix && !p.pre_splits && (!encode_cache_map16(&pre_k, p.kp, 1, p.prefix, width, kElems, kSlice) || !encode_cache_map16(&pre_v, p.vp, 1, p.prefix, width, kElems, kSlice)))
+  if (p.prefix && !p.pre_splits && (!encode_cache_map16(&pre_k, p.kp, 1, p.prefix, p.kvH, p.d, kElems, kSlice) || !encode_cache_map16(&pre_v, p.vp, 1, p.prefix, p.kvH, p.d, kElems, kSlice)))
     return cudaErrorInvalidValue;
-  if (p.capacity && (!encode_cache_map16(&own_k, p.ko, p.B, p.capacity, width, kElems, kSlice) || !encode_cache_map16(&own_v, p.vo, p.B, p.capacity, width, kElems, kSlice)))
+  if (p.capacity && (!encode_cache_map16(&own_k, p.ko, p.B, p.capacity, p.kvH, p.d, kElems, kSlice) || !encode_cache_map16(&own_v, p.vo, p.B, p.capacity, p.kvH, p.d, kElems, kSlice)))
     return cudaErrorInvalidValue;
   return launch_pdl(attn_shared_mma_kernel<T, D, ROWS>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kMT), smem, s, p.pre_splits != 0, pre_k, pre_v,
                     own_k, own_v, p, hgroups);
@@ -294,12 +293,8 @@ cudaError_t launch_d(cudaStream_t s, const SharedAttn& p, uint32_t rows) {
 }
 template <typename T>
 cudaError_t launch_t(cudaStream_t s, const SharedAttn& p, uint32_t rows) {
-  switch (p.d) {
-    case 32: return launch_d<T, 32>(s, p, rows);
-    case 64: return launch_d<T, 64>(s, p, rows);
-    case 128: return launch_d<T, 128>(s, p, rows);
-    default: return cudaErrorInvalidValue;
-  }
+  if (p.d > 128) return cudaErrorInvalidValue;
+  return p.d <= 32 ? launch_d<T, 32>(s, p, rows) : p.d <= 64 ? launch_d<T, 64>(s, p, rows) : launch_d<T, 128>(s, p, rows);
 }
 
 }  // namespace

@@ -1,4 +1,5 @@
-// The shared rows, once for every sequence: 16-bit types, heads of 64 and 128, on the 5th-generation tensor cores.
+// The shared rows, once for every sequence: 16-bit types, heads up to 128, on the 5th-generation tensor cores. Heads that are not 64 or 128
+// are filled up with zeros to the next of them by the copies.
 //
 // The query heads of a KV head and the sequences are one list of rows (row = sequence * G + head of the group). A CTA has two streams of
 // 128 rows each, one accumulator lane a row, and walks a part of the keys in tiles of 128. With more than 128 rows the streams are
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // CTAs of the same keys are neighbours
   const bool twice = COPIES > 1 || row_tiles == 1;  // one row tile: the streams have it both
-  const uint32_t pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
+  const uint32_t d = p.d, pairs = (row_tiles + 1) / 2, G = p.qH / p.kvH, R = p.B * G, tile = blockIdx.x % pairs * 2, g = blockIdx.x / pairs % p.kvH,
                  split = blockIdx.x / pairs / p.kvH;
   const uint32_t all = (p.prefix + kPreTile - 1) / kPreTile, first = split * p.pre_tiles, n = min(p.pre_tiles, all - first);  // tiles of keys
   // Q comes by TMA where the rows of a copy are whole sequences' heads, by the softmax warps otherwise; one stream's, where both have the
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         bar_expect_tx(full0 + 8 * s, SM::kTile);
 #pragma unroll
         for (uint32_t b = 0; b < D / 64; ++b)
-          tma_load_2d(s_u32(sm) + SM::kRing + s * SM::kTile + b * (kPreTile * 128), map, (int)(g * D + b * 64), (int)((first + it) * kPreTile), full0 + 8 * s);
+          tma_load_4d(s_u32(sm) + SM::kRing + s * SM::kTile + b * (kPreTile * 128), map, (int)(b * 64), (int)g, (int)((first + it) * kPreTile), 0, full0 + 8 * s);
       }
       ++j;
       return true;
@@ -220,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
 #pragma unroll
         for (uint32_t i = 0; i < 16; i += kRows) {
           const uint32_t r = (warp & 7) * 16 + i + lane / kLanes, row = row0 + r % kLanesOf, b = row / G;
-          const uint4 v = row < R ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + g * G + (row - b * G)) * D + qc))
-                                  : make_uint4(0, 0, 0, 0);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (row < R && qc < d) v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + g * G + (row - b * G)) * d + qc));
           *reinterpret_cast<uint4*>(sm + st * SM::kQ + (qc >> 6) * (kPreRows * 128) + r * 128 + ((((qc & 63) >> 3) ^ (r & 7)) << 4)) = v;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           }
         }
         const uint64_t at = ((uint64_t)split * p.kvH + g) * R + r;
-        *reinterpret_cast<float4*>(p.pre_o + at * D + e * 4) = acc;
+        if (e * 4 < d) *reinterpret_cast<float4*>(p.pre_o + at * d + e * 4) = acc;
         if (e == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(top, total);
       }
     } else if (there) {
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       for (uint32_t i = lane; i < 32 * (kPieces / 2); i += 32) {
         const uint32_t r = i / (kPieces / 2), e = half * (kPieces / 2) + i % (kPieces / 2);
         const uint4 v = *reinterpret_cast<const uint4*>(sums + piece(quarter * 32 + r, e));
-        if (row - lane + r < R) *reinterpret_cast<uint4*>(p.pre_o + (at0 + row - lane + r) * D + e * 4) = v;
+        if (row - lane + r < R && e * 4 < d) *reinterpret_cast<uint4*>(p.pre_o + (at0 + row - lane + r) * d + e * 4) = v;
       }
     }
   }
@@ -420,10 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
 template <typename T, int D, int COPIES>
 cudaError_t launch_copies(cudaStream_t s, const SharedAttn& p) {
   CUtensorMap mapQ{}, mapK, mapV;
-  const uint64_t width = (uint64_t)p.kvH * D;
-  if (!encode_tile_map16(&mapK, p.kp, p.prefix, width, kPreTile) || !encode_tile_map16(&mapV, p.vp, p.prefix, width, kPreTile)) return cudaErrorInvalidValue;
+  if (!encode_cache_map16(&mapK, p.kp, 1, p.prefix, p.kvH, p.d, 64, kPreTile) || !encode_cache_map16(&mapV, p.vp, 1, p.prefix, p.kvH, p.d, 64, kPreTile)) return cudaErrorInvalidValue;
   const uint32_t G = p.qH / p.kvH;
-  if (kPreRows / COPIES % G == 0 && !encode_query_map16(&mapQ, p.q, p.B, p.kvH, G, D, kPreRows / COPIES / G)) return cudaErrorInvalidValue;
+  if (kPreRows / COPIES % G == 0 && !encode_query_map16(&mapQ, p.q, p.B, p.kvH, G, p.d, kPreRows / COPIES / G)) return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(attn_shared_umma_kernel<T, D, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PreSmem<D>::kTotal);
   if (e != cudaSuccess) return e;
   const uint64_t row_tiles = ((uint64_t)p.B * (p.qH / p.kvH) + kPreRows - 1) / kPreRows;
@@ -442,8 +442,9 @@ cudaError_t launch_pre(cudaStream_t s, const SharedAttn& p) {
 }  // namespace
 
 cudaError_t launch_attn_shared_umma(cudaStream_t s, int dtype, const SharedAttn& p) {
-  if (dtype == 1) return p.d == 64 ? launch_pre<__half, 64>(s, p) : p.d == 128 ? launch_pre<__half, 128>(s, p) : cudaErrorInvalidValue;
-  if (dtype == 2) return p.d == 64 ? launch_pre<__nv_bfloat16, 64>(s, p) : p.d == 128 ? launch_pre<__nv_bfloat16, 128>(s, p) : cudaErrorInvalidValue;
+  if (p.d > 128) return cudaErrorInvalidValue;
+  if (dtype == 1) return p.d <= 64 ? launch_pre<__half, 64>(s, p) : launch_pre<__half, 128>(s, p);
+  if (dtype == 2) return p.d <= 64 ? launch_pre<__nv_bfloat16, 64>(s, p) : launch_pre<__nv_bfloat16, 128>(s, p);
   return cudaErrorInvalidValue;
 }
 

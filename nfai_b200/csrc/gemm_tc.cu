@@ -754,21 +754,22 @@ bool encode_tile_map16(CUtensorMap* map, const void* base, uint64_t rows, uint64
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint64_t rows, uint64_t K, uint32_t box_elems, uint32_t box_rows) {
+bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint64_t rows, uint64_t heads, uint64_t D, uint32_t box_elems,
+                        uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
-  if (!fn || (box_elems != 64 && box_elems != 32)) return false;
-  cuuint64_t dims[3] = {K, rows, seqs};
-  cuuint64_t strides[2] = {K * 2, rows * K * 2};
-  cuuint32_t box[3] = {box_elems, box_rows, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  if (!fn || D % 8 || (box_elems != 64 && box_elems != 32)) return false;
+  cuuint64_t dims[4] = {D, heads, rows, seqs};
+  cuuint64_t strides[3] = {D * 2, heads * D * 2, rows * heads * D * 2};
+  cuuint32_t box[4] = {box_elems, 1, box_rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             box_elems == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool encode_query_map16(CUtensorMap* map, const void* base, uint64_t B, uint64_t kvH, uint64_t G, uint64_t D, uint32_t seqs) {
   EncodeTiledFn fn = encode_fn();
-  if (!fn || D % 64 || G > 256 || seqs > 256) return false;
+  if (!fn || D % 8 || G > 256 || seqs > 256) return false;
   cuuint64_t dims[4] = {D, G, kvH, B};
   cuuint64_t strides[3] = {D * 2, G * D * 2, kvH * G * D * 2};
   cuuint32_t box[4] = {64, (cuuint32_t)G, 1, seqs};

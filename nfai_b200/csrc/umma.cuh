@@ -13,9 +13,11 @@ bool encode_tile_map16(CUtensorMap* map, const void* base, uint64_t rows, uint64
 // rows x box_blocks blocks of 64 elements, blocks outermost; 128-byte swizzle, zero fill outside. Coordinates: 0, row, block, layer.
 bool encode_stack_map16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t layers, uint64_t stride, uint32_t box_rows,
                         uint32_t box_blocks);
-// Tensor map of `seqs` caches of [rows][K] 16-bit elements one behind the other: box = box_elems elements (64, 128-byte swizzle, or 32,
-// 64-byte swizzle) x box_rows rows of one of them; zero fill outside. Coordinates: element, row, cache.
-bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint64_t rows, uint64_t K, uint32_t box_elems, uint32_t box_rows);
+// Tensor map of `seqs` caches of [rows][heads][D] 16-bit elements (D a multiple of 8) one behind the other: box = box_elems elements (64,
+// 128-byte swizzle, or 32, 64-byte swizzle) of one head x box_rows rows of one of them; zero fill outside the head and behind the rows.
+// Coordinates: element of the head, head, row, cache.
+bool encode_cache_map16(CUtensorMap* map, const void* base, uint64_t seqs, uint64_t rows, uint64_t heads, uint64_t D, uint32_t box_elems,
+                        uint32_t box_rows);
 // Tensor map of queries [B][kvH][G][D], 16-bit: box = 64 elements of the G heads of a KV head of `seqs` sequences, 128-byte swizzle, zero
 // fill outside. Coordinates: element, 0, KV head, sequence.
 bool encode_query_map16(CUtensorMap* map, const void* base, uint64_t B, uint64_t kvH, uint64_t G, uint64_t D, uint32_t seqs);
@@ -86,13 +88,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(map), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
 

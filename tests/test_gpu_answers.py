@@ -206,7 +206,9 @@ ATTN_SIZES = [  # B, qH, kvH, d, P, cap, lens
     (70, 8, 8, 40, 513, 2, [b % 3 for b in range(70)]), (13, 20, 4, 64, 1000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 900, 5, [5, 4, 3, -1, 1, 0]),
     (200, 8, 8, 40, 1513, 2, [b % 3 for b in range(200)]), (13, 20, 4, 64, 8000, 9, [b % 10 for b in range(13)]), (6, 48, 8, 128, 3900, 5, [5, 4, 3, -1, 1, 0]),
     (33, 16, 1, 128, 2000, 100, [3 * b for b in range(33)]), (80, 20, 4, 64, 1900, 130, [b * 2 % 131 for b in range(80)]), (50, 32, 8, 64, 640, 17, [-1] * 49 + [3]),
-    (90, 24, 4, 128, 2100, 100, [b + 11 for b in range(90)])]
+    (90, 24, 4, 128, 2100, 100, [b + 11 for b in range(90)]), (40, 20, 4, 72, 1500, 21, [b % 22 for b in range(40)]), (100, 8, 2, 8, 9000, 5, [b % 7 - 1 for b in range(100)]),
+    (36, 16, 1, 120, 2500, 30, [b % 31 for b in range(36)]), (64, 8, 2, 32, 2200, 20, [b % 21 for b in range(64)]), (250, 8, 2, 32, 700, 9, [b % 10 for b in range(250)]),
+    (3, 24, 8, 104, 2900, 40, [40, 0, 7]), (20, 12, 2, 136, 1500, 20, [b for b in range(20)])]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
@@ -232,7 +234,7 @@ def test_attention_peaked_scaled_and_repeated(cuda_ctx, kind, B, d, P):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("B,d,P,G", [(3, 64, 200, 2), (24, 64, 1500, 2), (24, 128, 1500, 2), (3, 32, 300, 2), (80, 64, 1500, 4), (80, 128, 1500, 8)])
+@pytest.mark.parametrize("B,d,P,G", [(3, 64, 200, 2), (24, 64, 1500, 2), (24, 128, 1500, 2), (3, 32, 300, 2), (80, 64, 1500, 4), (80, 128, 1500, 8), (80, 40, 3100, 8), (30, 88, 3100, 3)])
 def test_attention_values_that_are_not_finite(cuda_ctx, kind, B, d, P, G):
     """Keys that are -infinity towards a query have no weight; a row with no others is not a number; neither is one that sees a NaN; and
     other rows are as they were."""
