@@ -7,7 +7,7 @@
 // tile of keys. While one stream forms its weights the tensor pipe works for the other:
 //   warp 16  K and V tiles by TMA into a ring of 128-byte swizzled slots, in the order in which they are multiplied
 //   warp 17  one lane issues S(0), S(1), then for every unit (stream, tile) u: O += P(u) V, S(u + 2) = Q K^T, with P in tensor memory where S(u)
-//            was and V as it lies (its rows run along N). (A warp for each stream was no faster, 76 us for 72 with 64 sequences behind 32768
+//            was (for heads up to 64 there is room for a third unit: S(u + 3)) and V as it lies (its rows run along N). (A warp for each stream was no faster, 76 us for 72 with 64 sequences behind 32768
 //            rows: the streams fell into step and wanted the same units at the same time.)
 //   warp 18  sees the ring's slots fill, in order, and arrives with the softmax warps on the barrier that warp 17 waits for: waiting for the
 //            tiles itself cost that warp 600 of 3700 cycles in which nothing was multiplied
@@ -17,6 +17,11 @@
 // for the others: a row's exponentials are then spread over the schedulers, whose warps each see 32 lanes only.
 // At the end sums of weighted values, maxima and sums of weights go to scratch line by line, by way of shared memory, where streams and
 // copies of the same rows are joined; attn_shared_join_kernel joins the parts with those of the own rows.
+// Bound by the softmax warps: a tile of 128 keys takes them 1850 cycles, of which the unit for exponentials works 1024. A fourth of the weights
+// is computed as a polynomial for that reason. 128 sequences of 32 heads of 64 behind 20000 rows: 48.4 us, with a third unit 45.6, with the
+// polynomial 44.2 (for an eighth of the weights 44.4, a third 45.0); 64 of 32 of 128 behind 32768: 68.9, polynomial 68.2. For those the
+// kernel itself takes 42 us, 0.82 PFLOP/s, where 1.68 have been measured: the two products of a tile take 1290 cycles, 4 us at the end
+// are the sums' way to memory. With few rows it is bound by memory: 5 sequences of 32 heads of 64 behind 100003 rows 40 us, 5.1 TB/s.
 // Scores are products of the 16-bit queries as they are; the scale goes into the exponent's multiply-add. A row's sums are rescaled only
 // when its maximum has grown by more than 2^8 since the last time.
 #include <type_traits>
@@ -41,9 +46,10 @@ struct PreSmem {
   static constexpr uint32_t kTile = kPreTile * D * 2;
   static constexpr uint32_t kSlots = D == 64 ? 12 : 5;
   static constexpr uint32_t kQ = kPreRows * D * 2;  // of one stream
+  static constexpr uint32_t kPlaces = D == 64 ? 3 : 2;  // units that have their scores or weights in tensor memory
   static constexpr uint32_t kRing = 2 * kQ;
   static constexpr uint32_t kBarOff = kRing + kSlots * kTile;
-  static constexpr uint32_t kSwapOff = kBarOff + 256;  // [stream][half][row]: maxima of the halves of a row, later their sums, maxima and sums
+  static constexpr uint32_t kSwapOff = kBarOff + 512;  // [stream][half][row]: maxima of the halves of a row, later their sums, maxima and sums
   static constexpr uint32_t kTotal = kSwapOff + 4 * kPreRows * 4;
 };
 static_assert(PreSmem<64>::kTotal <= 232448 && PreSmem<128>::kTotal <= 232448, "shared memory of a CTA");
@@ -53,6 +59,23 @@ __device__ __forceinline__ float p_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x of two numbers (at most 2^7 of them, NaN stays NaN, below -126.5 gives 0) without the unit for it: x = n + f with a whole n and f in
+// [-1/2, 1/2], 2^f as a polynomial of degree 5 (fitted to the least relative error by weighted least squares on Chebyshev points; in
+// float32 off by 2.2e-7 at most), and 2^n put together from its exponent.
+__device__ __forceinline__ void poly_ex2(float& a, float& b) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+  auto both = [](float v) { return pair(v, v); };
+  constexpr float kWhole = 12583039.f;  // 1.5 * 2^23 + 127: adding it leaves n + 127 in the last bits
+  const uint64_t x = pair(a, b), t = add2(x, both(kWhole)), f = fma2(add2(t, both(-kWhole)), both(-1.f), x);
+  uint64_t y = fma2(f, both(0.0013276472454890609f), both(0.009675540961325169f));
+  y = fma2(y, f, both(0.05550713092088699f));
+  y = fma2(y, f, both(0.24022120237350464f));
+  y = fma2(y, f, both(0.6931469440460205f));
+  y = fma2(y, f, both(1.0000001192092896f));
+  unpair(t, a, b);
+  unpair(fma2(y, pair(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)), 0), a, b);
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -77,17 +100,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
                                                                        const __grid_constant__ CUtensorMap mapV, const SharedAttn p,
                                                                        const uint32_t row_tiles) {
   using SM = PreSmem<D>;
-  constexpr uint32_t kSP = 128, kO = 256;  // columns of tensor memory: a stream's scores and weights, its sums behind both streams' scores
+  // columns of tensor memory: NB places for the scores and weights of a unit, the streams' sums behind them
+  constexpr uint32_t NB = SM::kPlaces, kSP = 128, kO = NB * kSP;
+  static_assert(kO + 2 * D <= 512, "tensor memory");
   constexpr uint32_t kTypes = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u);
   constexpr uint32_t kKeys = kPreTile / COPIES, kMine = kKeys / 2, kLanesOf = kPreRows / COPIES;  // of a copy: keys, a thread's keys, lanes
   extern __shared__ __align__(1024) unsigned char pre_raw[];
   unsigned char* const sm = pre_raw;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + SM::kBarOff);
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SM::kSlots + 7);
   const uint32_t full0 = s_u32(bars), empty0 = s_u32(bars + SM::kSlots), q_ready = s_u32(bars + 2 * SM::kSlots);
-  auto s_ready = [&](uint32_t st) { return q_ready + 8 + 8 * st; };
-  auto p_ready = [&](uint32_t st) { return q_ready + 24 + 8 * st; };
-  auto pv_done = [&](uint32_t st) { return q_ready + 40 + 8 * st; };
+  // A wait knows a phase by its parity only. So whoever waits for one of these sees every phase of it: the softmax warps their stream's
+  // units (every second one), warps 17 and 18 all of them.
+  constexpr uint32_t NS = NB % 2 ? 2 * NB : NB;
+  auto s_ready = [&](uint32_t u) { return q_ready + 8 + 8 * (u % NS); };
+  auto s_turn = [&](uint32_t u) { return u / NS & 1; };
+  auto p_ready = [&](uint32_t u) { return q_ready + 8 + 8 * NS + 8 * (u % NB); };
+  auto p_turn = [&](uint32_t u) { return u / NB & 1; };
+  auto pv_last = [&](uint32_t st) { return q_ready + 8 + 8 * (NS + NB) + 8 * st; };  // the stream's last product with values is done
+  // Every one of them, for a wait that is seldom needed: who waits for that of the stream's tile `it` knows that the one before is done
+  // and that the one after has not been issued.
+  auto pv_done = [&](uint32_t st) { return pv_last(2) + 8 * st; };
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SM::kSlots + NS + NB + 5);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // CTAs of the same keys are neighbours
   const bool twice = COPIES > 1 || row_tiles == 1;  // one row tile: the streams have it both
@@ -104,9 +137,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       bar_init(empty0 + 8 * i, 1);
     }
     bar_init(q_ready, whole_q ? 2 : 17);
+    for (uint32_t i = 0; i < NS; ++i) bar_init(s_ready(i), 1);
+    for (uint32_t i = 0; i < NB; ++i) bar_init(p_ready(i), 9);
     for (uint32_t i = 0; i < 2; ++i) {
-      bar_init(s_ready(i), 1);
-      bar_init(p_ready(i), 9);
+      bar_init(pv_last(i), 1);
       bar_init(pv_done(i), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -148,11 +182,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       ++j;
       return true;
     };
-    if (twice) {  // K0 K1, V0 K2, V1 K3, ..
-      load(&mapK, 0);
-      if (n > 1 && ok) load(&mapK, 1);
+    if (twice) {  // K0 K1, V0 K2, V1 K3, .. (K0 K1 K2, V0 K3, ..)
+      for (uint32_t u = 0; u < NB && u < n && ok; ++u) load(&mapK, u);
       for (uint32_t u = 0; u < n && ok; ++u)
-        if (!load(&mapV, u) || (u + 2 < n && !load(&mapK, u + 2))) break;
+        if (!load(&mapV, u) || (u + NB < n && !load(&mapK, u + NB))) break;
     } else {  // K0 V0, K1 V1, ..
       for (uint32_t it = 0; it < n && ok; ++it)
         if (!load(&mapK, it) || !load(&mapV, it)) break;
@@ -164,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     constexpr uint32_t idesc_o = kTypes | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((kPreRows >> 4) << 24);
     const uint32_t base = s_u32(sm);
     // the place in the ring's order of the keys of unit u, and of its values
-    auto keys_of = [&](uint32_t u) { return twice ? (u < 2 ? u : 2 * u - 1) : (u >> 1) * 2; };
-    auto values_of = [&](uint32_t u) { return twice ? (u + 2 < units ? 2 * u + 2 : units + u) : (u >> 1) * 2 + 1; };
+    auto keys_of = [&](uint32_t u) { return twice ? (u < NB ? u : 2 * u - NB + 1) : (u >> 1) * 2; };
+    auto values_of = [&](uint32_t u) { return twice ? min(u + NB, units) + u : (u >> 1) * 2 + 1; };
     auto scores = [&](uint32_t u) {
       const uint32_t st = u & 1, s = keys_of(u) % SM::kSlots;
       if (elect_one()) {
@@ -173,30 +206,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
 #pragma unroll
         for (uint32_t kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (kPreRows * 128) + (kk & 3) * 32;
-          umma_f16(tmem + st * kSP, smem_desc_sw128(q_s + off), smem_desc_sw128(k_s + off), idesc_s, kk != 0);
+          umma_f16(tmem + u % NB * kSP, smem_desc_sw128(q_s + off), smem_desc_sw128(k_s + off), idesc_s, kk != 0);
         }
         if (twice || st) umma_commit(empty0 + 8 * s);
-        umma_commit(s_ready(st));  // (arrives when everything issued before is done, this stream's product before included)
+        umma_commit(s_ready(u));
       }
     };
     ok = all_wait_for(q_ready, 0);  // Q, and the first keys' tiles
     fence_after();
-    for (uint32_t u = 0; u < 2 && u < units && ok; ++u) scores(u);
+    for (uint32_t u = 0; u < NB && u < units && ok; ++u) scores(u);
     for (uint32_t u = 0; u < units && ok; ++u) {
       const uint32_t st = u & 1, it = u >> 1, j = values_of(u);  // it: the stream's own count
-      const bool more = u + 2 < units;
-      if (!(ok = all_wait_for(p_ready(st), it & 1))) break;  // the weights, the values' tile and the next scores' keys
+      if (!(ok = all_wait_for(p_ready(u), p_turn(u)))) break;  // the weights, the values' tile and the next scores' keys
       fence_after();
       if (elect_one()) {
         const uint32_t s = j % SM::kSlots, v_s = base + SM::kRing + s * SM::kTile;
 #pragma unroll
         for (uint32_t kk = 0; kk < kPreTile / 16; ++kk)
-          umma_f16_ta(tmem + kO + st * D, tmem + st * kSP + kk * 8, smem_desc_mn_sw128(v_s + kk * 2048, kPreTile * 128), idesc_o, (it | kk) != 0);
+          umma_f16_ta(tmem + kO + st * D, tmem + u % NB * kSP + kk * 8, smem_desc_mn_sw128(v_s + kk * 2048, kPreTile * 128), idesc_o, (it | kk) != 0);
         if (twice || st) umma_commit(empty0 + 8 * s);
-        if (!more) umma_commit(pv_done(st));
+        if (NB > 2) umma_commit(pv_done(st));
+        if (u + 2 >= units) umma_commit(pv_last(st));
       }
       // (the weights lie where the next scores go: products of one thread run in their order)
-      if (more) scores(u + 2);
+      if (u + NB < units) scores(u + NB);
     }
   } else if (warp == 18) {
     // All slots, each phase, in the ring's order: a wait knows a phase by its parity only.
@@ -205,13 +238,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     auto see = [&](uint32_t upto) {  // the first `upto` tiles have arrived
       for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1);
     };
-    see(min(tiles, twice ? 2u : 1u));
+    see(min(tiles, twice ? NB : (NB - 1) / 2 * 2 + 1));
     if (ok && lane == 0) bar_arrive(q_ready);
     for (uint32_t u = 0; u < units && ok; ++u) {
-      const uint32_t st = u & 1, it = u >> 1;
-      see(min(tiles, twice ? 2 * u + 4 : (it + 1) * 2 + 1));
-      if (it && ok) ok = all_wait_for(p_ready(st), (it - 1) & 1);  // (the phase before has ended: this arrival is for the next)
-      if (ok && lane == 0) bar_arrive(p_ready(st));
+      see(min(tiles, twice ? 2 * u + NB + 2 : (u + NB) / 2 * 2 + 1));
+      if (u >= NB && ok) ok = all_wait_for(p_ready(u), p_turn(u - NB));  // (the phase before has ended: this arrival is for the next)
+      if (ok && lane == 0) bar_arrive(p_ready(u));
     }
   } else {
     if (!whole_q) {  // the rows as they are, each piece of 16 bytes to its place under the swizzle
@@ -232,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     }
     const uint32_t quarter = warp & 3, half = warp >> 2 & 1, place = quarter * 32 + lane, copy = quarter / (4 / COPIES);
     const uint32_t col0 = copy * kKeys + half * kMine, row = row0 + place % kLanesOf;
-    const uint32_t lanes = tmem + (quarter * 32u << 16), cS = st * kSP, cO = kO + st * D;
+    const uint32_t lanes = tmem + (quarter * 32u << 16), cO = kO + st * D;
     const uint32_t tiles = twice ? (n + 1 - st) / 2 : n;  // of this stream
     const bool there = __any_sync(0xffffffffu, row < R);  // else this warp's exponentials are left out
     const float c = p.scale2, growth = kGrowth / c, floor = c > 1.f ? -1e38f / c : -1e38f;
@@ -251,11 +283,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     };
     float m = 0.f, l = 0.f;  // m: of the scores as they are
     for (uint32_t it = 0; it < tiles; ++it) {
-      // these scores are there, and the product with the tile before's values is done (a warp that gave up still meets the other one)
-      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(st), it & 1));
+      // These scores are there, and the products that were issued before them are done: with NB = 2 that of this stream's last tile is
+      // one of them, with NB = 3 that of the tile before. (A warp that gave up still meets the other one.)
+      const uint32_t u = 2 * it + st, cS = u % NB * kSP;
+      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(u), s_turn(u)));
       if (!there) {
         __syncwarp();
-        if (lane == 0) bar_arrive(p_ready(st));
+        if (lane == 0) bar_arrive(p_ready(u));
         continue;
       }
       const uint32_t n0 = (first + (twice ? it * 2 + st : it)) * kPreTile + col0;
@@ -287,6 +321,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           if (it) {
             const float f = p_ex2((m - top) * c);
             l *= f;
+            if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1));
+            fence_after();
 #pragma unroll 1
             for (uint32_t k = half * (D / 2); k < (half + 1) * (D / 2); k += 16) {
               uint32_t o[16];
@@ -305,8 +341,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           for (uint32_t j = 0; j < kPart; ++j) {
             float a, b;
             unpair(fma2(pair(__uint_as_float(s[(k * kPart + j) * 2]), __uint_as_float(s[(k * kPart + j) * 2 + 1])), c2, minus_m), a, b);
-            a = p_ex2(a);
-            b = p_ex2(b);
+            if (j % 4 == 3) {
+              poly_ex2(a, b);
+            } else {
+              a = p_ex2(a);
+              b = p_ex2(b);
+            }
             sum[j & 1] = add2(sum[j & 1], pair(a, b));
             w[j] = pack2(a, b, T());
           }
@@ -337,9 +377,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       tmem_st_wait();
       fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(p_ready(st));
+      if (lane == 0) bar_arrive(p_ready(u));
     }
-    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), 0));
+    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_last(st), 0));
     if (there) {
       swap[half * kPreRows + place] = l;
       meet();

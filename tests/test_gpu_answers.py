@@ -220,7 +220,8 @@ def test_attention(cuda_ctx, kind, case):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("B,d,P", [(2, 64, 100), (24, 64, 1500), (24, 128, 1500), (3, 32, 300)])
+@pytest.mark.parametrize("B,d,P", [(2, 64, 100), (24, 64, 1500), (24, 128, 1500), (3, 32, 300), (24, 64, 15000), (24, 128, 15000), (6, 64, 60000), (6, 128, 60000), (100, 64, 9000),
+                                   (100, 128, 9000), (40, 32, 9000)])
 def test_attention_peaked_scaled_and_repeated(cuda_ctx, kind, B, d, P):
     """Scores far apart (a few keys have all the weight, maxima grow along the walk), another scale, and twice with the same bits."""
     s = attn_args(kind, B, 8, 2, d, P, 200, [(37 * b) % 201 for b in range(B)], seed=B + d, spread=6.0)
