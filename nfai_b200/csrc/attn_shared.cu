@@ -302,11 +302,14 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   if (shared) {
     const bool umma = dtype != 0;
     a.pre_warps = umma ? 0 : R <= 16 ? 2 : R <= 32 || d > 64 ? 4 : 8;
-    // On tcgen05 one CTA on every SM, each with two tiles of 128 rows (sequence, head of the group), or one tile twice; on the CUDA cores
-    // 16 warps, of 8 rows each, an SM. (36 rows in 5 warps of one CTA rather than 8: 48 us for 39; of heads of 128, 4 warps or 8: 33 | 38.)
-    // As many keys for one as for the others.
+    // On tcgen05 a CTA has an SM and two tiles of 128 rows (sequence, head of the group), or one tile twice. Up to 64 rows it waits for
+    // memory, which 120 SMs keep busy while the own rows are walked on the others: 5 sequences of 32 over 8 heads of 64 behind 100003 rows
+    // 40.4 us, on all SMs 42.8; 3 of 16 over 1 of 128 behind 200000 30.2 | 38.0; 16 of 16 of 64 behind 30000 28.9 | 30.5. More rows are bound
+    // by what the SMs do (128 sequences of 32 over 8 of 64 behind 20000 on 112 SMs 49.8, all 44.3). On the CUDA cores 16 warps, of 8 rows
+    // each, an SM (36 rows in 5 warps of one CTA rather than 8: 48 us for 39; of heads of 128, 4 warps or 8: 33 | 38). As many keys for one
+    // CTA as for the others.
     const uint64_t row_tiles = umma ? (R + kPreRows - 1) / kPreRows : (R + a.pre_warps * 8 - 1) / (a.pre_warps * 8);
-    const uint64_t groups = (umma ? (row_tiles + 1) / 2 : row_tiles) * kvH, room = umma ? 148 : 148 * 16 / a.pre_warps;
+    const uint64_t groups = (umma ? (row_tiles + 1) / 2 : row_tiles) * kvH, room = umma ? (R <= 64 ? 120 : 148) : 148 * 16 / a.pre_warps;
     const uint32_t tile = umma ? kPreTile : attn_shared_rows_keys(d), tiles = (prefix + tile - 1) / tile;
     uint64_t parts = room / groups;
     parts = parts < 1 ? 1 : parts > kMaxPreSplits ? kMaxPreSplits : parts;
