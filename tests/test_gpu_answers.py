@@ -208,7 +208,8 @@ ATTN_SIZES = [  # B, qH, kvH, d, P, cap, lens
     (33, 16, 1, 128, 2000, 100, [3 * b for b in range(33)]), (80, 20, 4, 64, 1900, 130, [b * 2 % 131 for b in range(80)]), (50, 32, 8, 64, 640, 17, [-1] * 49 + [3]),
     (90, 24, 4, 128, 2100, 100, [b + 11 for b in range(90)]), (40, 20, 4, 72, 1500, 21, [b % 22 for b in range(40)]), (100, 8, 2, 8, 9000, 5, [b % 7 - 1 for b in range(100)]),
     (36, 16, 1, 120, 2500, 30, [b % 31 for b in range(36)]), (64, 8, 2, 32, 2200, 20, [b % 21 for b in range(64)]), (250, 8, 2, 32, 700, 9, [b % 10 for b in range(250)]),
-    (3, 24, 8, 104, 2900, 40, [40, 0, 7]), (20, 12, 2, 136, 1500, 20, [b for b in range(20)])]
+    (3, 24, 8, 104, 2900, 40, [40, 0, 7]), (20, 12, 2, 136, 1500, 20, [b for b in range(20)]), (2, 8, 2, 64, 300, 0, [0, 5]), (2, 8, 2, 64, 0, 0, [3, 0]),
+    (30, 8, 2, 64, 3000, 0, [0] * 29 + [-1]), (100, 16, 4, 128, 2000, 0, [b % 2 for b in range(100)])]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
@@ -475,6 +476,43 @@ def test_on_another_stream_behind_its_work_and_captured(cuda_ctx):
     step(1)
     torch.cuda.synchronize()
     assert torch.equal(a["out"].view(torch.int16), want[2].view(torch.int16))
+
+
+def test_two_calls_at_once(cuda_ctx):
+    """Calls of one context on two streams, eager and as two graphs, each with its scratch: what they give one after the other."""
+    jobs = [attn_args(kind, 70, 32, 8, 64, 1900, 90, [(7 * b + i) % 91 for b in range(70)], seed=i) for i, kind in enumerate(("f16", "f32"))]
+    rules = rules_args(9, 50000, 500, 30, 3, seed=8)
+    devs = [rules_dev(rules) for _ in jobs]
+    for s, dev in zip(jobs, devs):
+        attn_call(cuda_ctx, s)
+        rules_call(cuda_ctx, rules, dev)
+    want = [(s["out"].clone(), dev["out"].clone()) for s, dev in zip(jobs, devs)]
+    streams, graphs = [torch.cuda.Stream() for _ in jobs], []
+
+    def both(go):
+        for s, dev in zip(jobs, devs):
+            s["out"].fill_(5.0), dev["out"].fill_(5.0)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in range(len(jobs)):
+                go(i)
+        torch.cuda.synchronize()
+        for s, dev, (a, b) in zip(jobs, devs, want):
+            assert torch.equal(s["out"], a) and torch.equal(dev["out"], b)
+
+    def calls(i, stream):
+        attn_call(cuda_ctx, jobs[i], stream=stream)
+        rules_call(cuda_ctx, rules, devs[i], stream=stream)
+    both(lambda i: calls(i, streams[i].cuda_stream))
+    for i, s in enumerate(streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=s):
+            calls(i, torch.cuda.current_stream().cuda_stream)
+
+    def replay(i):
+        with torch.cuda.stream(streams[i]):
+            graphs[i].replay()
+    both(replay)
 
 
 def test_two_contexts_from_two_threads(cuda_ctx):
