@@ -72,6 +72,12 @@ internal static unsafe partial class Native
     [DllImport(Lib)] internal static extern int nfai_model_tune(IntPtr model, int which, int mode, int rowsPerWarp, int depth, int ctasPerSm);
     [DllImport(Lib)] internal static extern int nfai_model_set_prefetch(IntPtr model, ulong lookaheadBytes, ulong extraBytes, int mode);
     [DllImport(Lib)] internal static extern int nfai_op_attn_decode_static(IntPtr ctx, float* q, void* kcache, void* vcache, int kvDType, uint seq, uint qH, uint kvH, uint d, float* outp);
+    // several answers to one prompt, one step of them at a time: device pointers; stream Zero waits, a cudaStream_t is enqueued to
+    [DllImport(Lib)] internal static extern int nfai_rope_frequencies(uint dims, double ropeBase, int scaling, double factor, double a, double b, uint trained, double* freqs, out float magnitude);
+    [DllImport(Lib)] internal static extern int nfai_op_rope_rows(IntPtr ctx, void* x, int xDType, ulong xStride, uint rows, uint qH, uint kvH, uint d, uint dims, int layout, double* freqs, float magnitude, int* positions, int* slots, void* qOut, void* kCache, void* vCache, int outDType, ulong cacheRows, IntPtr stream);
+    [DllImport(Lib)] internal static extern int nfai_op_attn_shared(IntPtr ctx, void* q, void* kPrefix, void* vPrefix, uint prefix, void* kOwn, void* vOwn, uint capacity, int* lens, int dtype, uint batch, uint qH, uint kvH, uint d, float scale, void* outp, void* scratch, nuint scratchBytes, IntPtr stream);
+    [DllImport(Lib)] internal static extern nuint nfai_op_attn_shared_scratch_bytes(int dtype, uint batch, uint qH, uint kvH, uint d, uint prefix, uint capacity);
+    [DllImport(Lib)] internal static extern int nfai_op_logit_rules(IntPtr ctx, float* logits, uint rows, uint V, uint* history, uint historyStride, int* historyLen, float* repetition, float* frequency, float* presence, int* biasStart, uint* biasIds, float* bias, uint nBias, uint* masks, uint nMasks, int* maskRows, float* outp, IntPtr stream);
     [DllImport(Lib)] internal static extern int nfai_profile_kernel(IntPtr model, int which, int iters, out float avgMs, out ulong bytesPerLaunch);
     [DllImport(Lib)] internal static extern int nfai_step_launches(IntPtr model, out int launches);
     [DllImport(Lib)] internal static extern int nfai_step_kernels(IntPtr model, out int kernels);

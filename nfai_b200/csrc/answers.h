@@ -65,7 +65,7 @@ struct SharedAttn {
   float* own_ml = nullptr;            // [own_splits][B * qH][2]
   uint32_t pre_splits = 0, pre_tiles = 0;  // parts of the shared rows, tiles of keys per CTA; 0: they are walked like a sequence's own
   uint32_t own_splits = 1, own_least = 64; // parts of a sequence's keys at most, and keys of a part at least
-  bool joined = false;                // more than one partial result per row: they go to scratch and a last kernel joins them
+  bool joined = false;                // partial results go to scratch and a last kernel joins them (else the CTAs of a row do, if it has more than one)
   uint32_t* err = nullptr;            // device word of the context; may be null
 };
 // What the sizes alone decide: which kernels run, into how many parts, and what scratch they need.

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p
   const uint32_t hg = blockIdx.x % hgroups, g = blockIdx.x / hgroups % p.kvH, b = blockIdx.x / hgroups / p.kvH;
   const uint32_t h0 = g * G + hg * NR, nh = min((uint32_t)NR, G - hg * NR);
   const Walk walk = walk_of(p, b, blockIdx.y);
-  if (walk.idle || blockIdx.y >= walk.parts) return leave(p);
+  if (walk.idle || (p.joined && blockIdx.y >= walk.parts)) return leave(p);
   {
     const T* const qg = reinterpret_cast<const T*>(p.q) + ((uint64_t)b * p.qH + h0) * d;
     for (uint32_t i = tid; i < NR * d; i += kST) q[i] = i < nh * d ? to_float(qg[i]) * p.scale2 : 0.f;
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p
     q[i] = a;  // (the queries have been used)
   }
   __syncthreads();
-  leave_rows<T, kST, false>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l, nullptr);
+  leave_rows<T, kST, 4>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l, K);  // (the groups' sums have been used)
 }
 
 template <typename T, int NR>
@@ -157,7 +157,8 @@ cudaError_t launch_any(cudaStream_t s, const SharedAttn& p) {
   cudaError_t e = cudaFuncSetAttribute(attn_shared_any_kernel<T, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const uint32_t hgroups = (p.qH / p.kvH + NR - 1) / NR;
-  return launch_pdl(attn_shared_any_kernel<T, NR>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kST), smem, s, p.pre_splits != 0, p, hgroups);
+  return launch_pdl_cluster(attn_shared_any_kernel<T, NR>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kST), dim3(1, p.joined ? 1 : p.own_splits, 1), smem, s,
+                            p.pre_splits != 0, p, hgroups);
 }
 // The join of partial results, a row of the output (sequence, query head) per WARPS warps. A lane has four dimensions (UNITS times) of a
 // part; where LANES of them are a whole row, the warp has 32 / LANES parts at once. Eight parts are on their way at a time.
@@ -322,11 +323,18 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
   // CTAs for every SM twice over (the CUDA cores' four times) where the keys go so far. A part has 128 keys at least where the walk of the
   // shared rows hides the time it takes (8 sequences behind 2011 rows: 11.4 us, 11.9 with 64, 12.3 with 32; 5 behind 100003: 46.3, 45.5,
-  // 44.6), 32 where it is all there is (2 sequences of 340 keys: 5.9 us, 6.2 with 64, 6.1 with 128).
+  // 44.6), 32 where it is all there is (2 sequences of 340 keys and a join: 5.9 us, 6.2 with 64, 6.1 with 128).
   a.own_least = !a.tensor ? 64 : shared ? 128 : 32;
   uint64_t parts = (148 * (a.tensor ? 2 : 4) + groups - 1) / groups;
   if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
+  // Up to 8 CTAs of a sequence's heads join their parts among each other, as a cluster, and with a few more wanted it is 8: a launch less is
+  // worth more to a host that makes the call than what the kernel then takes longer. 2 sequences of 32 over 8 heads of 64 with 428 keys: 11.3 us
+  // a call from Python, with a join 13.4; in a graph 6.2 | 6.0 (4 sequences with 1128: 7.9 | 7.4; one with 10500, 37 parts: 16.5 | 10.5). The CUDA
+  // cores take too long with fewer CTAs (9 of 8 over 2 of 32 with 1512, 24 parts: 11.0 | 8.5), and behind a walk of the shared rows a cluster
+  // waits for room (8 sequences behind 2011 rows: 14.8 | 11.4).
+  constexpr uint32_t kMoreWanted = 24;
+  if (a.tensor && !shared && parts > kMostCtas && parts <= kMoreWanted) parts = kMostCtas;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -339,7 +347,7 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   // make up for the wait, without a join | with one: 256 sequences of 32 over 8 heads of 64 behind 1500 rows 55.7 | 61.7 us, 128 behind 8000
   // 49.2 | 52.6, 100 of 128 behind 4000 42.6 | 47.7, 64 of 128 behind 16000 (16 parts) 57.7 | 57.7, behind 32768 (18) 72.0 | 68.4; with one
   // head a KV head, 300 of 16 of 64 behind 1500, 52.7 | 44.9. On the CUDA cores it takes registers that the walk needs: 10.8 us for 8.4.
-  a.joined = a.own_splits > 1 || (a.pre_splits && (!a.tensor || G < 4 || a.pre_splits > kFewParts));
+  a.joined = a.own_splits > (shared ? 1 : kMostCtas) || (a.pre_splits && (!a.tensor || G < 4 || a.pre_splits > kFewParts));
   a.pre_ml = take(a.pre_splits * rows * 8);
   a.own_ml = take(a.joined ? a.own_splits * rows * 8 : 0);
   a.pre_o = take(a.pre_splits * rows * d * 4);

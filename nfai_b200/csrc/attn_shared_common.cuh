@@ -16,6 +16,7 @@ namespace shared_attn {
 constexpr uint32_t kMaxOwnSplits = 148;   // parts a sequence's keys are cut into
 constexpr uint32_t kMaxPreSplits = 148;   // CTAs that the shared rows are divided among
 constexpr uint32_t kFewParts = 16;        // parts of the shared rows that the kernel for the own rows adds by itself
+constexpr uint32_t kMostCtas = 8;         // of a sequence's heads that join their parts in a cluster
 constexpr uint32_t kPreRows = 128;        // (sequence, head of the group) of a CTA that walks the shared rows
 constexpr uint32_t kPreTile = 128;        // ... and its keys per tile
 
@@ -67,14 +68,23 @@ __device__ __forceinline__ uint64_t key_row(const SharedAttn& p, uint32_t b, uin
   return own ? (uint64_t)b * p.capacity + (t - shared) : (uint64_t)t;
 }
 
+// A number, or four, of another CTA of the cluster
+__device__ __forceinline__ float ld_far(const float* at, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(umma::s_u32(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
 // Everything a CTA does behind its walk: rows[j][d] (stride ld), m[j], l[j] of its query heads h0 .. h0 + nh - 1 are in shared memory,
-// all of it written and synchronised. The only part of a sequence's own keys is its result, after the parts of the shared rows have been
-// added to it where those have a kernel of their own and there are few (WITH_SHARED); others go to scratch for the join.
-// room: leave_room(..) floats of shared memory, free and aligned to 16 bytes.
-__host__ __device__ constexpr uint32_t leave_room(uint32_t rows, uint32_t threads) { return (rows * (kFewParts + 1) + 3) / 4 * 4 + threads * 4; }
-template <typename T, int THREADS, bool WITH_SHARED>
+// all of it written and synchronised. They go to scratch for the join, or the CTAs of a sequence's heads, which are a cluster then, join
+// them among each other, with what the shared rows gave where those have a kernel of their own: every CTA a share of the output.
+// AHEAD: parts that are asked for at once. room: leave_room(..) floats of shared memory, free and aligned to 16 bytes.
+__host__ __device__ constexpr uint32_t leave_room(uint32_t rows, uint32_t threads) { return (rows * (kFewParts + kMostCtas + 1) + 3) / 4 * 4 + threads * 4; }
+template <typename T, int THREADS, int AHEAD>
 __device__ __forceinline__ void leave_rows(const SharedAttn& p, uint32_t b, uint32_t h0, uint32_t nh, const Walk& w, uint32_t split,
-                                           const float* rows, uint32_t ld, const float* m, float* l, float* room) {
+                                           const float* rows, uint32_t ld, const float* m, const float* l, float* room) {
   const uint32_t tid = threadIdx.x, d = p.d, d4 = d / 4, row0 = b * p.qH + h0;
   if (p.joined) {
     const uint64_t at = (uint64_t)split * p.B * p.qH + row0;
@@ -96,63 +106,70 @@ __device__ __forceinline__ void leave_rows(const SharedAttn& p, uint32_t b, uint
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + j * d + e) = *reinterpret_cast<const float4*>(y);
     else *reinterpret_cast<uint2*>(out + j * d + e) = *reinterpret_cast<const uint2*>(y);
   };
-  const uint32_t n = p.pre_splits;
-  if (!WITH_SHARED || !n) {
+  const uint32_t n = p.pre_splits, ctas = p.own_splits, all = n + ctas;  // parts: the shared rows', then the CTAs' own
+  if (all == 1) {
     for (uint32_t i = tid; i < nh * d4; i += THREADS) {
       const uint32_t j = i / d4, e = (i - j * d4) * 4;
       store(j, e, *reinterpret_cast<const float4*>(rows + j * ld + e), w.n ? 1.0f / l[j] : 0.f);  // (no keys at all: zeros; none with a weight: 0 * infinity)
     }
     return;
   }
-  pdl_wait();  // the parts of the shared rows are there; of a part the CTA's heads stand one after the other
+  if (ctas > 1) umma::cluster_sync();
+  if (n) pdl_wait();  // (of a part of the shared rows the CTA's heads stand one after the other)
   const uint32_t G = p.qH / p.kvH, g = h0 / G, warp = tid >> 5, lane = tid & 31;
   const uint64_t R = (uint64_t)p.B * G, step = p.kvH * R, at0 = (uint64_t)g * R + (uint64_t)b * G + (h0 - g * G);
-  float* const f = room;                                           // [nh][n + 1]: the parts' factors and that of the own rows
-  float4* const half = reinterpret_cast<float4*>(room + (nh * (n + 1) + 3) / 4 * 4);
-  for (uint32_t j = warp; j < nh; j += THREADS / 32) {  // lane n: the own rows
+  float* const f = room;                // [nh][all]: the parts' factors
+  float* const inv = room + nh * all;   // [nh]
+  float4* const half = reinterpret_cast<float4*>(room + (nh * (all + 1) + 3) / 4 * 4);
+  for (uint32_t j = warp; j < nh; j += THREADS / 32) {
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(p.pre_ml + (lane * step + at0 + j) * 2));
-    if (lane == n) ml = make_float2(m[j], l[j]);
+    else if (ctas == 1 && lane == n) ml = make_float2(m[j], l[j]);
+    else if (lane < all) ml = make_float2(ld_far(m + j, lane - n), ld_far(l + j, lane - n));
     const float top = warp_max(ml.x), ref = top == -INFINITY ? 0.f : top, x = exp2f(ml.x - ref);
-    if (lane <= n) f[j * (n + 1) + lane] = x;
+    if (lane < all) f[j * all + lane] = x;
     // (a part without weights: nothing of it counts, but a sum that is not a number does)
     const float total = warp_sum(x != 0.f || ml.y != ml.y ? x * ml.y : 0.f);
-    if (lane == 0) l[j] = total;
+    if (lane == 0) inv[j] = w.n || n ? 1.0f / total : 0.f;
   }
   __syncthreads();
-  // a thread has four dimensions of a head; where threads are left, they share its parts
-  const uint32_t units = nh * d4, sets = units < THREADS ? THREADS / units : 1u, set = tid / units, first = sets > 1 ? tid - set * units : tid;
-  for (uint32_t i = first; i < units && set < sets; i += sets > 1 ? units : THREADS) {
-    const uint32_t j = i / d4, e = (i - j * d4) * 4;
-    const float* const fj = f + j * (n + 1);
+  // This CTA's share: a thread has four dimensions of a head; where threads are left, they share its parts.
+  const uint32_t units = nh * d4, from = split * units / ctas, mine = (split + 1) * units / ctas - from;
+  const uint32_t sets = mine && mine < THREADS ? THREADS / mine : 1u, set = sets > 1 ? tid / mine : 0u, first = sets > 1 ? tid - set * mine : tid;
+  for (uint32_t i = first; i < mine && set < sets; i += sets > 1 ? mine : THREADS) {
+    const uint32_t j = (from + i) / d4, e = (from + i - j * d4) * 4;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float x, float4 v) {
-      if (x != 0.f) { acc.x = fmaf(x, v.x, acc.x); acc.y = fmaf(x, v.y, acc.y); acc.z = fmaf(x, v.z, acc.z); acc.w = fmaf(x, v.w, acc.w); }
-    };
-    for (uint32_t k0 = set; k0 < n; k0 += 8 * sets) {
-      float4 v[8];
+    for (uint32_t k0 = set; k0 < all; k0 += AHEAD * sets) {
+      float4 v[AHEAD];
 #pragma unroll
-      for (uint32_t k = 0; k < 8; ++k)
-        if (k0 + k * sets < n) v[k] = __ldcg(reinterpret_cast<const float4*>(p.pre_o + ((k0 + k * sets) * step + at0 + j) * d + e));
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k)
-        if (k0 + k * sets < n) add(fj[k0 + k * sets], v[k]);
-    }
-    if (set == 0) add(fj[n], *reinterpret_cast<const float4*>(rows + j * ld + e));
-    if (sets > 1) half[tid] = acc;
-    else store(j, e, acc, 1.0f / l[j]);
-  }
-  if (sets > 1) {
-    __syncthreads();
-    if (tid < units) {
-      float4 acc = half[tid];
-      for (uint32_t k = 1; k < sets; ++k) {
-        const float4 v = half[k * units + tid];
-        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      for (uint32_t k = 0; k < AHEAD; ++k) {
+        const uint32_t part = k0 + k * sets;
+        if (part < n) v[k] = __ldcg(reinterpret_cast<const float4*>(p.pre_o + (part * step + at0 + j) * d + e));
+        else if (ctas == 1 && part == n) v[k] = *reinterpret_cast<const float4*>(rows + j * ld + e);
+        else if (part < all) v[k] = umma::ld_cluster(umma::s_u32(rows + j * ld + e), part - n);
       }
-      const uint32_t j = tid / d4;
-      store(j, (tid - j * d4) * 4, acc, 1.0f / l[j]);
+#pragma unroll
+      for (uint32_t k = 0; k < AHEAD; ++k) {
+        const uint32_t part = k0 + k * sets;
+        const float x = part < all ? f[j * all + part] : 0.f;
+        if (x != 0.f) {
+          acc.x = fmaf(x, v[k].x, acc.x); acc.y = fmaf(x, v[k].y, acc.y); acc.z = fmaf(x, v[k].z, acc.z); acc.w = fmaf(x, v[k].w, acc.w);
+        }
+      }
     }
+    if (sets > 1) half[tid] = acc;
+    else store(j, e, acc, inv[j]);
+  }
+  if (ctas > 1) umma::cluster_sync();  // (nobody leaves while others read its rows; and what follows is behind a barrier)
+  else __syncthreads();
+  if (sets > 1 && tid < mine) {
+    float4 acc = half[tid];
+    for (uint32_t k = 1; k < sets; ++k) {
+      const float4 v = half[k * mine + tid];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    const uint32_t j = (from + tid) / d4;
+    store(j, (from + tid - j * d4) * 4, acc, inv[j]);
   }
 }
 

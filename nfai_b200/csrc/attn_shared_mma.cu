@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
   const uint32_t hg = blockIdx.x % hgroups, g = blockIdx.x / hgroups % p.kvH, b = blockIdx.x / hgroups / p.kvH, split = blockIdx.y;
   const uint32_t h0 = g * G + hg * ROWS, nh = min((uint32_t)ROWS, G - hg * ROWS);
   const Walk walk = walk_of(p, b, split);
-  if (walk.idle || split >= walk.parts) return leave(p);
+  if (walk.idle || (p.joined && split >= walk.parts)) return leave(p);  // (a cluster's CTA without keys takes part in the join)
   // slices of the shared rows first, then of the sequence's own: none has keys of both
   const uint32_t shared = p.pre_splits ? 0u : p.prefix, cut = min(max(shared, walk.t0), walk.t1);
   const uint32_t before = (cut - walk.t0 + kSlice - 1) / kSlice, slices = before + (walk.t1 - cut + kSlice - 1) / kSlice;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
     }
   }
   __syncthreads();
-  leave_rows<T, kMT, true>(p, b, h0, nh, walk, split, rows, PL, M, L, part);  // (the warps' rows have been used)
+  leave_rows<T, kMT, 8>(p, b, h0, nh, walk, split, rows, PL, M, L, part);  // (the warps' rows have been used)
 }
 
 template <typename T, int D, int ROWS>
@@ -284,8 +284,8 @@ cudaError_t launch_rows(cudaStream_t s, const SharedAttn& p) {
     return cudaErrorInvalidValue;
   if (p.capacity && (!encode_cache_map16(&own_k, p.ko, p.B, p.capacity, p.kvH, p.d, kElems, kSlice) || !encode_cache_map16(&own_v, p.vo, p.B, p.capacity, p.kvH, p.d, kElems, kSlice)))
     return cudaErrorInvalidValue;
-  return launch_pdl(attn_shared_mma_kernel<T, D, ROWS>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kMT), smem, s, p.pre_splits != 0, pre_k, pre_v,
-                    own_k, own_v, p, hgroups);
+  return launch_pdl_cluster(attn_shared_mma_kernel<T, D, ROWS>, dim3(p.B * p.kvH * hgroups, p.own_splits), dim3(kMT), dim3(1, p.joined ? 1 : p.own_splits, 1),
+                            smem, s, p.pre_splits != 0, pre_k, pre_v, own_k, own_v, p, hgroups);
 }
 template <typename T, int D>
 cudaError_t launch_d(cudaStream_t s, const SharedAttn& p, uint32_t rows) {
