@@ -9,10 +9,12 @@
 // Bound by HBM: logits in, logits out, a bit a token for the mask. A CTA owns a slice of one row's vocabulary. One thread has the slice
 // copied into shared memory and, at the end, out of it; meanwhile all count what of the row's history falls into the slice (whole
 // numbers: the order of the additions makes no difference). A thread remembers which of its tokens were the first in their place: for
-// those it applies the penalties. The last listing of a bias is found among the lanes of a warp, or in the table, which is empty again. What
-// the mask takes away is overwritten last.
-// 48 rows of 128256: 9.3 us with nothing asked for (5.3 TB/s), 15 with 4000 tokens of history, 18 with that, biases, and masks for half of the
-// rows: issue slots, for the history in every slice and for the masks, are what it costs (50 % of them are used). Tried: penalties where
+// those it applies the penalties. The last listing of a bias is found among the lanes of a warp, or in the table, which is empty again.
+// The mask comes last: a lane has the bits of 32 tokens, which the warp then takes one lane's after the other, so that neighbouring lanes
+// write neighbouring tokens.
+// 48 rows of 128256: 9.5 us with nothing asked for (5.2 TB/s), 14.5 with 4000 tokens of history, 12.4 with a mask for every row (17.0 where a
+// thread had four neighbouring tokens: stores to the same banks), 16.6 with history, biases, and masks for half of the rows: issue slots for
+// the history in every slice are what it costs. Tried: 16 tokens of the history asked for at once (17.5 for 17.1), penalties where
 // the logits are stored (22.3: nearly every warp has a touched token and takes the path for all), one wave of slices twice as long
 // with the logits in registers (18.5), clusters of eight slices that share the history and add to one another's counts (21.7: 14.2 with
 // nothing asked for), a look at every token's count a second time (19.1).
@@ -28,8 +30,7 @@ namespace nfai {
 namespace {
 
 constexpr int kLT = 256;
-constexpr uint32_t kQuads = 6;
-constexpr uint32_t kLongest = kQuads * kLT * 4;  // tokens of a slice: 8 bytes of shared memory each, four CTAs to an SM
+constexpr uint32_t kLongest = 6144;  // tokens of a slice: 8 bytes of shared memory each, four CTAs to an SM
 constexpr uint32_t kShortest = 1024;
 constexpr uint32_t kSeen = 8;   // tokens of the history that a thread asks for at once
 constexpr uint32_t kKept = 32;  // ... and for which it remembers whether they were the first in their place
@@ -89,18 +90,19 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     bias = __ldg(p.bias + b0 + lane);
   }
   __syncthreads();  // the table is empty
-  uint32_t words[kQuads] = {};  // of the mask, for this thread's quads: looked at when the slice is there
-  if (masked) {
-#pragma unroll
-    for (uint32_t k = 0; k < kQuads; ++k) {
-      const uint32_t t = t0 + (k * kLT + tid) * 4;
-      if (t < t1) words[k] = __funnelshift_r(__ldg(mask + (t >> 5)), VEC && peel ? __ldg(mask + (min(t + 3, p.V - 1) >> 5)) : 0u, t & 31);
-    }
+  // A warp masks a stretch of the slice, a lane has the bits of 32 tokens of it (one: allowed, or not in the slice).
+  const uint32_t len = t1 - t0, chunks = (S + kLT - 1) / kLT, warp = tid >> 5;
+  static_assert(kLongest / kLT <= 32, "chunks of a warp");
+  uint32_t word = ~0u;
+  if (masked && lane < chunks && (warp * chunks + lane) * 32 < len) {
+    const uint32_t c = (warp * chunks + lane) * 32, t = t0 + c, w = t >> 5;
+    word = __ldg(mask + w);
+    if (t & 31) word = __funnelshift_r(word, __ldg(mask + min(w + 1, (p.V - 1) >> 5)), t & 31);
+    if (len - c < 32) word |= ~0u << (len - c);
   }
 
   // a token's place in the tables; another slice's, or no token at all: `len` or more. (Tokens in front have theirs behind the slice; they
   // are looked for apart, where there are any: the history is what costs instructions, twice for every slice.)
-  const uint32_t len = t1 - t0;
   auto in_front = [&](auto&& each) {
     for (uint32_t i = tid; i < n_hist; i += kLT) {
       const uint32_t t = __ldg(h + i);
@@ -130,25 +132,10 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
   }
   if (front && peel) in_front([&](uint32_t c, uint32_t) { atomicAdd(count + c, 1u); });
   const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0));  // the slice is there, and everything is counted
-  if (masked) {
-#pragma unroll
-    for (uint32_t k = 0; k < kQuads; ++k) {
-      const uint32_t c = (k * kLT + tid) * 4, g = c < len ? ~words[k] & 15u : 0u;
-      if (g == 15u) {
-        *reinterpret_cast<float4*>(value + c) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      } else if (g) {
-        if (g & 1) value[c] = -INFINITY;
-        if (g & 2) value[c + 1] = -INFINITY;
-        if (g & 4) value[c + 2] = -INFINITY;
-        if (g & 8) value[c + 3] = -INFINITY;
-      }
-    }
-  }
-  if (front && tid < peel && !open(tid)) value[S + tid] = -INFINITY;
   if (n_hist) {
     auto rule = [&](uint32_t c, uint32_t t) {  // whoever finds a count takes it and leaves none
       const uint32_t n = atomicExch(count + c, 0u);
-      if (!n || !open(t)) return;
+      if (!n) return;
       float a = value[c];
       a = a > 0.f ? __fdiv_rn(a, rep) : a * rep;
       value[c] = __fsub_rn(__fsub_rn(a, __fmul_rn(freq, (float)n)), pres);
@@ -170,7 +157,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     if (few) {
       if (tid < 32) {
         const uint32_t same = __match_any_sync(0xffffffffu, listed), c = cell(listed);
-        if (lane == 31 - __clz(same) && c != none && open(listed)) value[c] = __fadd_rn(value[c], bias);
+        if (lane == 31 - __clz(same) && c != none) value[c] = __fadd_rn(value[c], bias);
       }
     } else {
       for (uint32_t i = b0 + tid; i < b1; i += kLT) {
@@ -180,10 +167,19 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
       __syncthreads();
       for (uint32_t i = b0 + tid; i < b1; i += kLT) {
         const uint32_t t = __ldg(p.bias_ids + i), c = cell(t);
-        if (c != none && count[c] == i + 1 && open(t)) value[c] = __fadd_rn(value[c], __ldg(p.bias + i));
+        if (c != none && count[c] == i + 1) value[c] = __fadd_rn(value[c], __ldg(p.bias + i));
       }
     }
   }
+  if (masked) __syncthreads();  // the mask comes last
+  if (masked) {
+#pragma unroll 4
+    for (uint32_t i = 0; i < chunks; ++i) {
+      const uint32_t gone = ~__shfl_sync(0xffffffffu, word, i);
+      if (gone >> lane & 1) value[(warp * chunks + i) * 32 + lane] = -INFINITY;
+    }
+  }
+  if (front && tid < peel && !open(tid)) value[S + tid] = -INFINITY;
   if (!ok) {
     if (p.err && tid == 0) atomicOr(p.err, 4u);
     // the copy may still be on its way: a bounded time for it to end before its memory is used for something else
