@@ -439,7 +439,7 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
  * caches are rounded to 16 bits for the product with the values). scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
  * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
  * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. What the rows behind
- * lens[b] hold makes no difference. scratch (device memory, 256-byte aligned) is used until the work is done;
+ * lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory, 256-byte aligned) is used until the work is done;
  * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused). */
 int nfai_op_attn_shared(nfai_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,
                         const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,
