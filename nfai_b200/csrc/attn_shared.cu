@@ -294,10 +294,9 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   const uint64_t R = (uint64_t)B * G;  // rows of a KV head
   // The walk of the shared rows pays from a length on that makes up for its own two kernels. Measured, without | with it, 16-bit on either
   // side of the rule: 64 sequences of 8 KV heads of 64 behind 430 rows, 16 behind 900, 4 behind 2500 take the same, 32 of 2 of 32 behind
-  // 2200, 250 behind 500. float32: 16 sequences of
-  // 2 KV heads of 32 behind 1024 rows 12.0 | 10.1 us, 512: 8.4 | 9.8; 2 of 8 of 64 behind 2048: 15.4 | 12.2, 512: 8.5 | 10.0. One sequence
-  // gains from it in float32 only, whose other kernel keeps fewer loads on their way (8 KV heads of 128 behind 16384 rows 75.8 | 65.5, 4096:
-  // 27.2 | 28.8); in 16 bits that one is at the memory's rate (36000 rows: 82 us of 81).
+  // 2200, 250 behind 500. float32: 16 sequences of 2 KV heads of 32 behind 1024 rows 12.0 | 10.1 us, 512: 8.4 | 9.8; 2 of 8 of 64 behind 2048:
+  // 15.4 | 12.2, 512: 8.5 | 10.0. One sequence gains from it in float32 only, whose other kernel keeps fewer loads on their way (8 KV heads of
+  // 128 behind 16384 rows 75.8 | 65.5, 4096: 27.2 | 28.8); in 16 bits that one is at the memory's rate (130000 rows: 82 us of 81).
   const uint64_t work = (uint64_t)prefix * B * kvH * d;
   const bool shared = dtype != 0 ? B >= 2 && d <= 128 && (uint64_t)prefix >= 200 + 6000000 / ((uint64_t)B * kvH * d) : work >= (B == 1 ? 4000000 : 1200000);
   if (shared) {
@@ -328,13 +327,12 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   uint64_t parts = (148 * (a.tensor ? 2 : 4) + groups - 1) / groups;
   if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
-  // Up to 8 CTAs of a sequence's heads join their parts among each other, as a cluster, and with a few more wanted it is 8: a launch less is
-  // worth more to a host that makes the call than what the kernel then takes longer. 2 sequences of 32 over 8 heads of 64 with 428 keys: 11.3 us
-  // a call from Python, with a join 13.4; in a graph 6.2 | 6.0 (4 sequences with 1128: 7.9 | 7.4; one with 10500, 37 parts: 16.5 | 10.5). The CUDA
-  // cores take too long with fewer CTAs (9 of 8 over 2 of 32 with 1512, 24 parts: 11.0 | 8.5), and behind a walk of the shared rows a cluster
+  // Up to 8 CTAs of a sequence's heads join their parts among each other, as a cluster, and where more are wanted for few keys it is 8: a
+  // launch less is worth more to a host that makes the call than what the kernel then takes longer. 2 sequences of 32 over 8 heads of 64 with
+  // 428 keys: 11.3 us a call from Python, with a join 13.4; in a graph 6.2 | 6.0 (one with 628: 6.9 | 6.5; with 10500, 16.5 | 10.5). The CUDA
+  // cores take too long with fewer CTAs (9 of 8 over 2 of 32 with 1512: 11.0 | 8.5), and behind a walk of the shared rows a cluster
   // waits for room (8 sequences behind 2011 rows: 14.8 | 11.4).
-  constexpr uint32_t kMoreWanted = 24;
-  if (a.tensor && !shared && parts > kMostCtas && parts <= kMoreWanted) parts = kMostCtas;
+  if (a.tensor && !shared && parts > kMostCtas && keys <= kMostCtas * 128) parts = kMostCtas;
   a.own_splits = parts < 1 ? 1 : (uint32_t)parts;
   size_t off = 0;
   auto take = [&](size_t bytes) {
