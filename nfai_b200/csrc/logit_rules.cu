@@ -17,7 +17,8 @@
 // the history in every slice are what it costs. Tried: 16 tokens of the history asked for at once (17.5 for 17.1), penalties where
 // the logits are stored (22.3: nearly every warp has a touched token and takes the path for all), one wave of slices twice as long
 // with the logits in registers (18.5), clusters of eight slices that share the history and add to one another's counts (21.7: 14.2 with
-// nothing asked for), a look at every token's count a second time (19.1).
+// nothing asked for), a look at every token's count a second time (19.1), a plain copy and behind
+// it a CTA a row that has the touched tokens in a hash table (26.2).
 //
 // In front of SamplingUtils.TopP (NFAI.Models.Llama3/SamplingUtils.cs:5-33); the reference has no such rules.
 #include "answers.h"
