@@ -435,8 +435,10 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
 
 /* Attention of one token of each of B sequences: out[b][h] = sum_t softmax_t(scale q[b][h] . k_t) v_t, where t runs over the `prefix`
  * rows [prefix][kvH*d] that all share and over the first lens[b] of the sequence's own [B][capacity][kvH*d]. The shared rows are read
- * once for all. q and out are [B][qH*d]; everything is of `dtype` (any of the three), sums and weights are float32 (weights of 16-bit
- * caches are rounded to 16 bits for the product with the values). scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
+ * once for all. q and out are [B][qH*d]; everything is of `dtype` (any of the three), scores, weights and sums are float32. For the product
+ * with the values of 16-bit caches and heads up to 128 a weight is rounded: to the caches' type where the shared rows are walked for all
+ * (in float16 to steps of 2^-31 of the row's largest weight at the finest), to two terms of it elsewhere (steps of 2^-39). Which of both
+ * depends on the sizes, so a sequence alone and in a batch may differ in the last bit. scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
  * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
  * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. What the rows behind
  * lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory, 256-byte aligned) is used until the work is done;

@@ -7,8 +7,9 @@
 // TMA (as 16-byte copies of all lanes the addresses took more issue slots than the products: 85 against 80 us with 64 sequences behind
 // 32768 rows); at the end the warps are joined in shared memory. Rows behind the last that counts may come with a slice: their scores
 // are -infinity and their values are overwritten with zeros. Warps that walk whole parts one after the other, asking for the next while
-// they multiply this one's last, spare the joining but not the wait for the warp with one part more: 77 us for 68 with 256 sequences. A weight is split into two 16-bit terms (two products into one sum): the products wait for memory anyway, and nothing of
-// the weight is lost.
+// they multiply this one's last, spare the joining but not the wait for the warp with one part more: 77 us for 68 with 256 sequences.
+// A weight is split into two 16-bit terms (two products into one sum): the products wait for memory anyway. In float16 22 bits of it count,
+// down to 2^-40 of the row's largest (kLift), in bfloat16 16.
 // 256 sequences of 32 heads of 64 with 500 rows of their own (and 60 shared ones): 44.9 us, 5.9 TB/s; of 128, 64 sequences: 4.4 TB/s (512 CTAs, three
 // to an SM: the second wave is not full).
 #include "attn_shared_common.cuh"
@@ -22,6 +23,12 @@ using namespace umma;
 
 constexpr int kMW = 4, kMT = kMW * 32;
 constexpr uint32_t kSlice = 16;  // keys per slice
+// Weights are multiplied by 2^kLift before they are split (their sum has the factor too): float16, with 2^16 as its largest number, ends at
+// 2^-25, so that its second term then reaches down to 2^-40 of a row's largest weight. bfloat16 has float32's range.
+template <typename T>
+constexpr float kLift = 0.0f;
+template <>
+constexpr float kLift<__half> = 15.0f;
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a));
@@ -193,7 +200,8 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
       }
       float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[r]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(__fadd_ru(top, -kLift<T>), m[r]);  // (rounded up: no weight is above 2^kLift, however large the scores)
       const float ref = top == -INFINITY ? 0.f : top, f = s_ex2(m[r] - ref);
       m[r] = top;
       float e[4];

@@ -22,6 +22,8 @@
 // polynomial 44.2 (for an eighth of the weights 44.4, a third 45.0); 64 of 32 of 128 behind 32768: 68.9, polynomial 68.2. For those the
 // kernel itself takes 42 us, 0.82 PFLOP/s, where 1.68 have been measured: the two products of a tile take 1290 cycles, 4 us at the end
 // are the sums' way to memory. With few rows it is bound by memory: 5 sequences of 32 heads of 64 behind 100003 rows 40 us, 5.1 TB/s.
+// Weights are rounded to the caches' type, as the product takes both operands of one type and a second term would double its time: a result is
+// 1.05 to 1.4 times as far from the one in 64 bits as with weights of 32, where the rounding of the result is nearly all.
 // Scores are products of the 16-bit queries as they are; the scale goes into the exponent's multiply-add. A row's sums are rescaled only
 // when its maximum has grown by more than 2^8 since the last time.
 #include <type_traits>
@@ -40,6 +42,12 @@ using shared_attn::wait_for;
 
 constexpr int kSoftmax = 512, kThreads = kSoftmax + 96;
 constexpr float kGrowth = 8.0f;
+// Weights are multiplied by 2^kLift before they are rounded (the weights' sum has the factor too, and the maximum that goes to scratch is
+// lower by it). float16 ends at 2^-25: without the factor a key that is 2^-25 lighter than its row's heaviest counts for nothing, and 100 000 of
+// them behind a heavy one are 0.003 of the row. 2^(kGrowth + kLift) is within float16, whose largest number is 2^16. (2^4 and 2^11 rescale more
+// often: 64 sequences of 32 heads of 128 behind 32768 rows 71.2 us for 67.3.) bfloat16 has float32's range.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 template <int D>
 struct PreSmem {
@@ -60,7 +68,7 @@ __device__ __forceinline__ float p_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x of two numbers (at most 2^7 of them, NaN stays NaN, below -126.5 gives 0) without the unit for it: x = n + f with a whole n and f in
+// 2^x of two numbers (x up to 127, NaN stays NaN, below -126.5 gives 0) without the unit for it: x = n + f with a whole n and f in
 // [-1/2, 1/2], 2^f as a polynomial of degree 5 (fitted to the least relative error by weighted least squares on Chebyshev points; in
 // float32 off by 2.2e-7 at most), and 2^n put together from its exponent.
 __device__ __forceinline__ void poly_ex2(float& a, float& b) {
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     const uint32_t lanes = tmem + (quarter * 32u << 16), cO = kO + st * D;
     const uint32_t tiles = twice ? (n + 1 - st) / 2 : n;  // of this stream
     const bool there = __any_sync(0xffffffffu, row < R);  // else this warp's exponentials are left out
-    const float c = p.scale2, growth = kGrowth / c, floor = c > 1.f ? -1e38f / c : -1e38f;
+    const float c = p.scale2, growth = __fdiv_rd(kGrowth, c), floor = c > 1.f ? -1e38f / c : -1e38f;
     const uint64_t c2 = pair(c, c);
     float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff) + st * 2 * kPreRows;  // [half][place]
     auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(st * 4 + quarter + 1) : "memory"); };
@@ -281,7 +289,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           : "memory");
       return r != 0;
     };
-    float m = 0.f, l = 0.f;  // m: of the scores as they are
+    // m: the maximum that counts, of the scores as they are; ref: what their exponents are taken from. Both this and the limit on growth are
+    // rounded such that no weight is above 2^(kGrowth + kLift), however large the scores.
+    auto ref_of = [&](float top) { return __fadd_ru(__fmul_ru(top, c), -kLift<T>); };
+    float m = floor, ref = 0.f, l = 0.f;
     for (uint32_t it = 0; it < tiles; ++it) {
       // These scores are there, and the products that were issued before them are done: with NB = 2 that of this stream's last tile is
       // one of them, with NB = 3 that of the tile before. (A warp that gave up still meets the other one.)
@@ -317,9 +328,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         if (raise) {
           swap[half * kPreRows + place] = top;
           meet();
-          top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + place]), it ? m : floor);
+          top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + place]), m);
+          const float before = ref;
+          ref = ref_of(top);
           if (it) {
-            const float f = p_ex2((m - top) * c);
+            const float f = p_ex2(before - ref);
             l *= f;
             if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1));
             fence_after();
@@ -335,12 +348,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           m = top;
         }
         sum[0] = sum[1] = 0;
-        const uint64_t minus_m = pair(-m * c, -m * c);
+        const uint64_t minus_ref = pair(-ref, -ref);
         auto weights = [&](uint32_t k, uint32_t (&w)[kPart]) {
 #pragma unroll
           for (uint32_t j = 0; j < kPart; ++j) {
             float a, b;
-            unpair(fma2(pair(__uint_as_float(s[(k * kPart + j) * 2]), __uint_as_float(s[(k * kPart + j) * 2 + 1])), c2, minus_m), a, b);
+            unpair(fma2(pair(__uint_as_float(s[(k * kPart + j) * 2]), __uint_as_float(s[(k * kPart + j) * 2 + 1])), c2, minus_ref), a, b);
             if (j % 4 == 3) {
               poly_ex2(a, b);
             } else {
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         uint32_t w[kPart];
         weights(0, w);
         fence_before();  // (the other warp's scores may lie where this one's weights go: both have read theirs now)
-        if (either(top > m + growth) && !raise) {
+        if (either(top > __fadd_rd(m, growth)) && !raise) {
           raise = true;
           continue;
         }
@@ -385,9 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       meet();
       l += swap[(half ^ 1) * kPreRows + place];
     }
-    // Every score -infinity (a row's sum has the 1 of its maximum otherwise): as if there were no keys. A wait that gave up: NaN.
-    float2 ml = make_float2(m * c, l);
-    if (l < 0.5f) ml = make_float2(-INFINITY, 0.f);
+    // Every score -infinity: as if there were no keys. A wait that gave up: NaN.
+    float2 ml = make_float2(ref, l);
+    if (m <= floor && l < 0.5f) ml = make_float2(-INFINITY, 0.f);
     if (!ok) ml = make_float2(0.f, __uint_as_float(0x7fffffffu));
     // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
     // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,

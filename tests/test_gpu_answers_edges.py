@@ -1,0 +1,61 @@
+"""Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest. The helpers and the
+conventions on tolerances are those of test_gpu_answers.py."""
+import pytest
+
+from nfai_b200 import _lib
+
+from .test_gpu_answers import TYPES, U, at, attn_args, attn_call, half_step
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ---- attention: weights far below the heaviest --------------------------------------------------------------------------------
+def attn_want(s, scale=0.0):
+    """The definition in 64 bits, sum w |v| and sum |v|: [B][qH][d] each; rows of free places are zero."""
+    B, qH, kvH, d, P = s["B"], s["qH"], s["kvH"], s["d"], s["P"]
+    want, size, all_v = torch.zeros(3, B, qH, d, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(s["lens"].tolist()):
+        n = min(n, s["cap"])
+        if n < 0 or P + n == 0:
+            continue
+        k = torch.cat([s["kp"].double(), s["ko"][b, :n].double()]).view(-1, kvH, d).permute(1, 2, 0)
+        v = torch.cat([s["vp"].double(), s["vo"][b, :n].double()]).view(-1, kvH, d).permute(1, 0, 2)
+        w = torch.softmax(s["q"][b].double().view(kvH, qH // kvH, d) @ k * (scale or d ** -0.5), -1)
+        want[b], size[b], all_v[b] = ((x @ y).view(qH, d) for x, y in ((w, v), (w, v.abs()), (torch.ones_like(w), v.abs())))
+    return want, size, all_v
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("where", ["shared", "own"])
+@pytest.mark.parametrize("B,kvH,G,d,P,cap", [(1, 2, 4, 64, 2000, 900), (24, 8, 4, 64, 3000, 600), (24, 8, 4, 128, 3000, 600), (3, 8, 4, 64, 9000, 700), (9, 2, 3, 128, 6000, 300),
+                                             (70, 8, 8, 40, 2500, 300), (200, 8, 4, 64, 1500, 60), (2, 2, 2, 256, 900, 300), (4, 2, 2, 32, 200, 800)])
+def test_attention_many_light_keys_behind_a_heavy_one(cuda_ctx, kind, where, B, kvH, G, d, P, cap):
+    """One key takes nearly all of a row's weight and has a value of zero (the first token of many models); what the row gives are the others,
+    17.5 below it, a weight of 2^-25.2 of the heaviest each.
+
+    Queries of 1 and keys of 0 and of 17.5 / sqrt(d) rounded to three bits: all scores are exact. A weight is rounded to the caches' type (not float32):
+    half a step of its size, or of float16's smallest step, 2^-24 of a weight that has been multiplied by 2^7: 2^-32 of the heaviest.
+    Exponentials 8 u, sums of n keys n u, one rounding of the result."""
+    s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d)
+    heavy = float(torch.tensor(17.5 / d ** 0.5).to(torch.float8_e4m3fn))
+    s["q"].fill_(1.0), s["kp"].zero_(), s["ko"].zero_()
+    for v in (s["vp"], s["vo"]):
+        v.copy_(v.float().abs().clamp(0.25, 4.0) * 8192.0)
+    k, v = (s["kp"], s["vp"]) if where == "shared" else (s["ko"], s["vo"])
+    if where == "shared":
+        k[P // 3], v[P // 3] = heavy, 0.0
+    else:
+        k[:, 5], v[:, 5] = heavy, 0.0
+    for b, n in enumerate(s["lens"].tolist()):  # what lies behind a sequence's rows is no number
+        s["ko"][b, n:], s["vo"][b, n:] = float("nan"), float("inf")
+    attn_call(cuda_ctx, s)
+    want, size, all_v = attn_want(s)
+    kind = TYPES[kind][0]
+    n = P + cap
+    half = half_step(kind) if kind != torch.float32 else 0.0
+    floor = 2.0 ** -32 * all_v if kind == torch.float16 else 0.0
+    room = (8 * U + half + n * U) * size + floor + half_step(kind) * want.abs() + torch.finfo(kind).tiny
+    off = (s["out"].view(want.shape).double() - want).abs()
+    assert (room < 0.05 * want).all()  # (what is left out would be seen)
+    assert (off <= room).all(), (off / room).max().item()
