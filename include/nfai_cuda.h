@@ -440,8 +440,10 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
  * (in float16 to steps of 2^-31 of the row's largest weight at the finest), to two terms of it elsewhere (steps of 2^-39). Which of both
  * depends on the sizes, so a sequence alone and in a batch may differ in the last bit. scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
  * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
- * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. What the rows behind
- * lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory, 256-byte aligned) is used until the work is done;
+ * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. An infinite value gives an
+ * infinity of its sign to every row that has a weight for it (above 2^-126 of the row's largest), values of both infinities or a NaN give NaN;
+ * what an infinite value gives to a row without a weight for it is not said.
+ * What the rows behind lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory, 256-byte aligned) is used until the work is done;
  * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused). */
 int nfai_op_attn_shared(nfai_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,
                         const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,

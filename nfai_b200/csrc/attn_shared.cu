@@ -33,7 +33,7 @@ __device__ __forceinline__ void widen8(const T* at, float (&f)[8]) {
 }
 
 template <typename T, int NR>
-__global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p, const uint32_t hgroups) {
+__global__ void __launch_bounds__(kST) attn_shared_any_kernel(const __grid_constant__ SharedAttn p, const uint32_t hgroups) {
   extern __shared__ __align__(16) float sm_any[];
   const uint32_t d = p.d, kld = k_stride(d), d4 = d / 4, d8 = d / 8, G = p.qH / p.kvH;
   float* const q = sm_any;               // [NR][d]
@@ -141,13 +141,18 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const SharedAttn p
     for (int r = 0; r < NR; ++r) *reinterpret_cast<float4*>(K + (r * KG + kg) * d + chunk * 4) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
   }
   __syncthreads();
+  bool odd = false;
   for (uint32_t i = tid; i < NR * d; i += kST) {
     const uint32_t r = i / d, e = i - r * d;
     float a = 0.f;
     for (uint32_t k = 0; k < KG; ++k) a += K[(r * KG + k) * d + e];
     q[i] = a;  // (the queries have been used)
+    odd |= a != a;
   }
-  __syncthreads();
+  if (__syncthreads_or(odd)) {
+    mend_part<T, kST>(p, b, h0, nh, walk.t0, walk.t1, q, d, l);
+    __syncthreads();
+  }
   leave_rows<T, kST, 4>(p, b, h0, nh, walk, blockIdx.y, q, d, m, l, K);  // (the groups' sums have been used)
 }
 

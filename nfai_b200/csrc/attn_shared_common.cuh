@@ -68,6 +68,70 @@ __device__ __forceinline__ uint64_t key_row(const SharedAttn& p, uint32_t b, uin
   return own ? (uint64_t)b * p.capacity + (t - shared) : (uint64_t)t;
 }
 
+// ---- infinite values ----
+// A sum of weighted values comes out as no number where an infinite value meets a weight, or a term of one, that is 0 in the type of the
+// product: the second term of a weight that is exact, a key that belongs to another copy of the row, a weight that is too small for float16.
+// Weights are above 0, so infinities of one sign are the sum, and those of both signs or a NaN are none. Which it is follows from the column of
+// values alone; the kernels look at it again, for the keys of their part, where a row whose weights' sum is a number has such an element.
+// `acc` becomes NaN where one of the four is
+__device__ __forceinline__ void note_nan(float& acc, float4 v) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc) : "f"(v.x));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc) : "f"(v.y));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc) : "f"(v.z));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc) : "f"(v.w));
+}
+__device__ __forceinline__ bool is_sum(float l) { return l > 0.f && l < INFINITY; }
+// Of n values a `step` apart: 1: +infinity is among them, 2: -infinity, 4: NaN. For a whole warp.
+template <typename T>
+__device__ __forceinline__ uint32_t infinities(const T* v, uint64_t step, uint32_t n) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t f = 0;
+#pragma unroll 1
+  for (uint32_t t0 = 0; t0 < n && !__any_sync(0xffffffffu, f & 4); t0 += 128) {
+    float x[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) x[k] = t0 + k * 32 + lane < n ? to_float(v[(t0 + k * 32 + lane) * step]) : 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) f |= x[k] == INFINITY ? 1u : x[k] == -INFINITY ? 2u : x[k] != x[k] ? 4u : 0u;
+  }
+  return __reduce_or_sync(0xffffffffu, f);
+}
+__device__ __forceinline__ float infinite_sum(uint32_t f) { return f == 1 ? INFINITY : f == 2 ? -INFINITY : __uint_as_float(0x7fffffffu); }
+
+// The keys [t0, t1) of sequence b: rows[j][d] (stride ld) and l[j] of its nh query heads from h0 on, which are one KV head's, in shared memory.
+// For a whole CTA. (A function of its own: the kernels keep the registers that they have without it.)
+template <typename T, int THREADS>
+__device__ __noinline__ void mend_part(const SharedAttn& p, uint32_t b, uint32_t h0, uint32_t nh, uint32_t t0, uint32_t t1, float* rows, uint32_t ld,
+                                       const float* l) {
+  const uint32_t d = p.d, lane = threadIdx.x & 31, shared = p.pre_splits ? 0u : p.prefix, cut = min(max(shared, t0), t1);
+  const uint64_t step = (uint64_t)p.kvH * d, column = (uint64_t)(h0 / (p.qH / p.kvH)) * d;
+  for (uint32_t e = threadIdx.x >> 5; e < d; e += THREADS / 32) {
+    const bool odd = lane < nh && is_sum(l[lane]) && rows[lane * ld + e] != rows[lane * ld + e];
+    if (!__any_sync(0xffffffffu, odd)) continue;
+    const T* const vp = reinterpret_cast<const T*>(p.vp) + t0 * step + column + e;
+    const T* const vo = reinterpret_cast<const T*>(p.vo) + ((uint64_t)b * p.capacity + (max(cut, shared) - shared)) * step + column + e;
+    const uint32_t f = infinities(vp, step, cut - t0) | infinities(vo, step, t1 - cut);
+    if (odd) rows[lane * ld + e] = infinite_sum(f);
+  }
+}
+// The shared keys [t0, t1) of KV head g: rows [r0, r1) of part `split`, in scratch, written by this CTA (or, with one warp, by this warp).
+template <typename T>
+__device__ __noinline__ void mend_shared(const SharedAttn& p, uint32_t split, uint32_t g, uint32_t r0, uint32_t r1, uint32_t t0, uint32_t t1, uint32_t warp,
+                                         uint32_t warps) {
+  const uint32_t d = p.d, lane = threadIdx.x & 31;
+  const uint64_t at = ((uint64_t)split * p.kvH + g) * p.B * (p.qH / p.kvH), step = (uint64_t)p.kvH * d;
+  for (uint32_t e = warp; e < d; e += warps) {
+    uint32_t f = ~0u;  // not looked at yet
+    for (uint32_t r = r0; r < r1; r += 32) {
+      float* const o = p.pre_o + (at + r + lane) * d + e;
+      const bool odd = r + lane < r1 && is_sum(__ldcg(p.pre_ml + (at + r + lane) * 2 + 1)) && __ldcg(o) != __ldcg(o);
+      if (!__any_sync(0xffffffffu, odd)) continue;
+      if (f == ~0u) f = infinities(reinterpret_cast<const T*>(p.vp) + t0 * step + (uint64_t)g * d + e, step, t1 - t0);
+      if (odd) *o = infinite_sum(f);
+    }
+  }
+}
+
 // A number, or four, of another CTA of the cluster
 __device__ __forceinline__ float ld_far(const float* at, uint32_t rank) {
   uint32_t a;

@@ -97,7 +97,7 @@ constexpr size_t mma_smem() {  // the stages, or what the warps are joined in
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_constant__ CUtensorMap pre_k, const __grid_constant__ CUtensorMap pre_v,
                                                               const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v,
-                                                              const SharedAttn p, const uint32_t hgroups) {
+                                                              const __grid_constant__ SharedAttn p, const uint32_t hgroups) {
   using SH = Shape<D>;
   constexpr int NST = SH::kStages, R = ROWS / 8;
   extern __shared__ unsigned char mma_raw[];
@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
     if ((lane & 3) == 0) *reinterpret_cast<float2*>(ml + (warp * ROWS + row) * 2) = make_float2(m[r], l[r]);
   }
   __syncthreads();
+  float odd = 0.f;
   for (uint32_t i = tid; i < nh * (D / 4); i += kMT) {
     const uint32_t j = i / (D / 4), e = i % (D / 4) * 4;
     float2 w[kMW];
@@ -273,12 +274,16 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
       }
     }
     *reinterpret_cast<float4*>(rows + j * PL + e) = acc;
+    note_nan(odd, acc);
     if (e == 0) {
       M[j] = top;
       L[j] = sum;
     }
   }
-  __syncthreads();
+  if (__syncthreads_or(odd != odd)) {
+    mend_part<T, kMT>(p, b, h0, nh, walk.t0, walk.t1, rows, PL, L);
+    __syncthreads();
+  }
   leave_rows<T, kMT, 8>(p, b, h0, nh, walk, split, rows, PL, M, L, part);  // (the warps' rows have been used)
 }
 

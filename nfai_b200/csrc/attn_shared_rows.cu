@@ -40,7 +40,7 @@ __device__ __forceinline__ void cp16(float* dst, const float* src, bool there) {
 }
 
 template <int CHUNKS>
-__global__ void __launch_bounds__(256) attn_shared_rows_kernel(const SharedAttn p, const uint32_t row_tiles) {
+__global__ void __launch_bounds__(256) attn_shared_rows_kernel(const __grid_constant__ SharedAttn p, const uint32_t row_tiles) {
   using SH = RowsShape<CHUNKS>;
   constexpr uint32_t TK = SH::kKeys, NK = SH::kMine;
   extern __shared__ __align__(16) float rows_sm[];
@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(256) attn_shared_rows_kernel(const SharedAttn 
     }
     __syncthreads();  // the tile has been used: the next may land there
   }
+  float odd = 0.f;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -174,9 +175,13 @@ __global__ void __launch_bounds__(256) attn_shared_rows_kernel(const SharedAttn 
       unpair(o[r][c][0], y.x, y.y);
       unpair(o[r][c][1], y.z, y.w);
       *reinterpret_cast<float4*>(p.pre_o + at * d + e) = y;
+      note_nan(odd, y);
     }
     if (kg == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(m[r], l[r]);
   }
+  const bool mend = __any_sync(0xffffffffu, odd != odd);
+  __syncwarp();
+  if (mend) mend_shared<float>(p, split, g, row0 + warp * kRowsOf, min(R, row0 + (warp + 1) * kRowsOf), t0, t1, 0, 1);
 }
 
 template <int CHUNKS>

@@ -105,7 +105,7 @@ using umma::tmem_st;
 template <typename T, int D, int COPIES>
 __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __grid_constant__ CUtensorMap mapQ,
                                                                        const __grid_constant__ CUtensorMap mapK,
-                                                                       const __grid_constant__ CUtensorMap mapV, const SharedAttn p,
+                                                                       const __grid_constant__ CUtensorMap mapV, const __grid_constant__ SharedAttn p,
                                                                        const uint32_t row_tiles) {
   using SM = PreSmem<D>;
   // columns of tensor memory: NB places for the scores and weights of a unit, the streams' sums behind them
@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   pdl_launch_dependents();  // the own rows do not wait for the shared ones, only the join does
   const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
   bool ok = true;
+  float odd = 0.f;  // NaN: one is among the sums that this thread has written
 
   if (warp == 16) {
     if (whole_q && elect_one()) {
@@ -446,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         }
         const uint64_t at = ((uint64_t)split * p.kvH + g) * R + r;
         if (e * 4 < d) *reinterpret_cast<float4*>(p.pre_o + at * d + e * 4) = acc;
+        shared_attn::note_nan(odd, acc);
         if (e == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(top, total);
       }
     } else if (there) {
@@ -455,8 +457,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
 #pragma unroll 4
       for (uint32_t i = lane; i < 32 * (kPieces / 2); i += 32) {
         const uint32_t r = i / (kPieces / 2), e = half * (kPieces / 2) + i % (kPieces / 2);
-        const uint4 v = *reinterpret_cast<const uint4*>(sums + piece(quarter * 32 + r, e));
-        if (row - lane + r < R && e * 4 < d) *reinterpret_cast<uint4*>(p.pre_o + (at0 + row - lane + r) * d + e * 4) = v;
+        const float4 v = *reinterpret_cast<const float4*>(sums + piece(quarter * 32 + r, e));
+        if (row - lane + r < R && e * 4 < d) *reinterpret_cast<float4*>(p.pre_o + (at0 + row - lane + r) * d + e * 4) = v;
+        shared_attn::note_nan(odd, v);
       }
     }
   }
@@ -467,8 +470,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     }
   }
   fence_before();
-  __syncthreads();
+  const bool mend = __syncthreads_or(odd != odd);
   if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (mend)
+    shared_attn::mend_shared<T>(p, split, g, tile * kPreRows, min(R, (tile + 2) * kPreRows), first * kPreTile, min(p.prefix, (first + n) * kPreTile), warp,
+                                kThreads / 32);
 }
 
 template <typename T, int D, int COPIES>

@@ -1,4 +1,4 @@
-"""Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest. The helpers and the
+"""Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest, infinite values. The helpers and the
 conventions on tolerances are those of test_gpu_answers.py."""
 import pytest
 
@@ -59,3 +59,49 @@ def test_attention_many_light_keys_behind_a_heavy_one(cuda_ctx, kind, where, B, 
     off = (s["out"].view(want.shape).double() - want).abs()
     assert (room < 0.05 * want).all()  # (what is left out would be seen)
     assert (off <= room).all(), (off / room).max().item()
+
+
+# ---- attention: infinite values -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("B,kvH,G,d,P,cap", [(1, 2, 4, 64, 300, 70), (3, 2, 2, 32, 200, 30), (24, 8, 4, 64, 1500, 40), (24, 8, 4, 128, 1500, 40), (5, 8, 4, 64, 9000, 100),
+                                             (9, 2, 3, 128, 6000, 300), (80, 2, 8, 40, 3100, 60), (200, 8, 4, 64, 1500, 60), (2, 2, 2, 256, 400, 70), (12, 2, 2, 136, 3000, 9), (2, 2, 4, 64, 0, 900)])
+def test_attention_infinite_values(cuda_ctx, kind, B, kvH, G, d, P, cap):
+    """An infinite value gives an infinity to every row that sees its key, however light the key is there; infinities of both signs and a NaN
+    give NaN; elements without either are as they were, bit for bit."""
+    s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d)
+    s["q"] = s["q"].abs() + 0.5
+    own = s["vo"].view(B, cap, kvH, d)
+    if P:
+        # key P // 4 lies about 20 below the others: below 2^-25 of a weight, above 2^-126
+        s["kp"][P // 4] = -20.0 / (1.7 * d ** 0.5)
+    clean = dict(s, out=s["out"].clone())
+    attn_call(cuda_ctx, clean)
+    if P:
+        v = s["vp"].view(P, kvH, d)
+        v[P // 3, :, 1], v[P // 2, 0, 2] = float("inf"), float("-inf")
+        v[P // 4, 1, 3] = float("inf")
+        v[0, 0, 4], v[P - 1, 0, 4] = float("inf"), float("-inf")
+        v[P // 5, 1, 5], v[P // 2, 1, 5] = float("inf"), float("nan")
+    own[:, 0, 0, 6] = float("inf")
+    own[B - 1, 1, 1, 7] = float("-inf")
+    own[B // 2, 2, 0, d - 1], own[B // 2, 1, 0, d - 1] = float("inf"), float("-inf")
+    attn_call(cuda_ctx, s)
+    want = attn_want(s)[0]
+    bad = ~want.isfinite()
+    got = s["out"].view(want.shape).double()
+    assert bad.any() and torch.equal(got[bad].nan_to_num(0.5), want[bad].nan_to_num(0.5))
+    assert torch.equal(got[~bad], clean["out"].view(want.shape).double()[~bad])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("B,d,P", [(1, 64, 200), (24, 64, 1500), (24, 128, 1500), (5, 64, 9000), (3, 256, 200)])
+def test_attention_infinite_values_without_a_weight(cuda_ctx, kind, B, d, P):
+    """A row whose scores are all -infinity, or one of them NaN, stays NaN, also where its values are infinite."""
+    s = attn_args(kind, B, 8, 2, d, P, 20, [20] * B, seed=B + d)
+    s["q"] = s["q"].abs() + 0.5
+    s["kp"].view(P, 2, d)[:, 0] = float("-inf")
+    s["ko"].view(B, 20, 2, d)[:, :, 0] = float("-inf")
+    s["kp"].view(P, 2, d)[P // 2, 1] = float("nan")
+    s["vp"][P // 3] = float("inf")
+    attn_call(cuda_ctx, s)
+    assert s["out"].isnan().all()
