@@ -24,17 +24,17 @@ struct OnDevice {
 };
 
 // `stream` null: the context's stream, and the result is there on return; else the work is put on that stream.
-// waits: the kernels have waits that may give up, which they note in the context's word (calls on a stream before this one, too).
+// waits: the kernels have waits that may give up, which they note in a word of the context (calls on a stream before this one, too).
 cudaStream_t stream_of(nfai_ctx* c, void* stream) { return stream ? static_cast<cudaStream_t>(stream) : c->stream; }
 int finish(nfai_ctx* c, void* stream, cudaError_t launched, bool waits) {
   if (launched != cudaSuccess)
     return fail(c, launched == cudaErrorInvalidValue ? NFAI_ERR_ARG : NFAI_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(launched));
   if (stream) return NFAI_OK;
   uint32_t err = 0;
-  if (waits) CU(c, cudaMemcpyAsync(&err, c->dev_err, 4, cudaMemcpyDeviceToHost, c->stream));
+  if (waits) CU(c, cudaMemcpyAsync(&err, c->answers_note(), 4, cudaMemcpyDeviceToHost, c->stream));
   CU(c, cudaStreamSynchronize(c->stream));
   if (!err) return NFAI_OK;
-  CU(c, cudaMemsetAsync(c->dev_err, 0, 4, c->stream));
+  CU(c, cudaMemsetAsync(c->answers_note(), 0, 4, c->stream));
   return fail(c, NFAI_ERR_TIMEOUT, "a bounded device-side wait gave up");
 }
 bool known_dtype(int t) { return t == NFAI_F32 || t == NFAI_F16 || t == NFAI_BF16; }
@@ -124,7 +124,7 @@ int nfai_op_logit_rules(nfai_ctx* c, const float* logits, uint32_t rows, uint32_
   p.history = history; p.history_stride = history ? history_stride : 0; p.history_len = history_len;
   p.repetition = repetition; p.frequency = frequency; p.presence = presence;
   p.bias_start = bias_start; p.bias_ids = bias_ids; p.bias = bias; p.n_bias = n_bias;
-  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->dev_err;
+  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->answers_note();
   return finish(c, stream, launch_logit_rules(stream_of(c, stream), p), true);
 }
 
@@ -166,7 +166,8 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   p.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)d)) * 1.4426950408889634);
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
   p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
-  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined; p.err = c->dev_err;
+  p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined;
+  p.err = c->answers_note();
   return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan), true);
 }
 

@@ -1788,7 +1788,10 @@ int nfai_op_gemm(nfai_ctx* c, const void* A, const void* W, int dtype, uint32_t 
   if (rc) return rc;
   uint32_t err = 0;
   CU(c, cudaMemcpy(&err, c->dev_err, 4, cudaMemcpyDeviceToHost));
-  if (err) return fail(c, NFAI_ERR_TIMEOUT, "a bounded wait inside the tensor-core GEMM gave up");
+  if (err) {
+    CU(c, cudaMemset(c->dev_err, 0, 4));  // (said once: the exchange's operators read the same word)
+    return fail(c, NFAI_ERR_TIMEOUT, "a bounded wait inside the tensor-core GEMM gave up");
+  }
   return NFAI_OK;
 }
 

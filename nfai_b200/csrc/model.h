@@ -36,7 +36,12 @@ struct nfai_ctx {
   cudaEvent_t stage_ev[kStageSlots] = {nullptr, nullptr};
   int stage_next = 0;
   uint32_t* pin_small = nullptr;  // pinned scratch for tokens / state read-back (256 bytes)
-  uint32_t* dev_err = nullptr;    // device word for error bits of kernels that run outside a model step
+  // 64 device words: 0 error bits of kernels that run outside a model step, whose calls clear it; 4 answers_note(); 8 a sampled token; 16, 18
+  // epoch and ticket of the exchange's operators; 32.. a step state for them
+  uint32_t* dev_err = nullptr;
+  // Error bits of attention over shared rows and rules on logits. They may be enqueued on a stream, with other operators between them and the
+  // call that reports them, so no other call touches this word.
+  uint32_t* answers_note() const { return dev_err + 4; }
   TpComm* tp = nullptr;
   bool pdl = true;
   bool use_graph = true;

@@ -1,10 +1,14 @@
 """Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest, infinite values. The helpers and the
 conventions on tolerances are those of test_gpu_answers.py."""
+import os
+import shutil
+import subprocess
+
 import pytest
 
-from nfai_b200 import _lib
+from nfai_b200 import build
 
-from .test_gpu_answers import TYPES, U, at, attn_args, attn_call, half_step
+from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -105,3 +109,18 @@ def test_attention_infinite_values_without_a_weight(cuda_ctx, kind, B, d, P):
     s["vp"][P // 3] = float("inf")
     attn_call(cuda_ctx, s)
     assert s["out"].isnan().all()
+
+
+# ---- a wait that gave up ------------------------------------------------------------------------------------------------------
+def test_a_wait_that_gave_up_is_told_by_the_next_call_that_waits(tmp_path):
+    """Also with other operators in between, by nobody else, and once; what others left in their word is not taken for it. The program writes
+    the words as a kernel that gave up does."""
+    gxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else shutil.which("g++")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(build._nvcc())))
+    lib, exe = build.build(), str(tmp_path / "answers_note")
+    subprocess.run([gxx, "-std=c++17", "-I", os.path.join(root, "nfai_b200", "csrc"), "-I", os.path.join(root, "include"), "-I", os.path.join(cuda, "include"),
+                    os.path.join(root, "tests", "cabi", "answers_note.cpp"), "-o", exe, "-L", os.path.dirname(lib), "-lnfai_cuda",
+                    "-Wl,-rpath," + os.path.dirname(lib), "-L", os.path.join(cuda, "lib64"), "-lcudart_static", "-lpthread", "-ldl", "-lrt"], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr)
