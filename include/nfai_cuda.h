@@ -443,8 +443,9 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
  * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. An infinite value gives an
  * infinity of its sign to every row that has a weight for it (above 2^-126 of the row's largest), values of both infinities or a NaN give NaN;
  * what an infinite value gives to a row without a weight for it is not said.
- * What the rows behind lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory, 256-byte aligned) is used until the work is done;
- * nfai_op_attn_shared_scratch_bytes gives the size (0 for sizes that are refused). */
+ * What the rows behind lens[b] hold makes no difference. Pointers to elements are aligned to 16 bytes. scratch (device memory,
+ * 256-byte aligned) is used until the work is done; nfai_op_attn_shared_scratch_bytes gives a size that serves these sizes and every smaller
+ * batch, prefix and capacity (0 for sizes that are refused). */
 int nfai_op_attn_shared(nfai_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,
                         const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,
                         uint32_t d, float scale, void* out, void* scratch, size_t scratch_bytes, void* stream);

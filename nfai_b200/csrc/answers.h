@@ -78,6 +78,8 @@ struct SharedPlan {
   size_t pre_o = 0, pre_ml = 0, own_o = 0, own_ml = 0, total = 0;  // byte offsets
 };
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity);
+// Scratch that serves these sizes and every smaller batch, prefix and capacity: grows with each of them, as a plan's own does not.
+size_t shared_attn_scratch(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity);
 // the shared rows, partial results into pre_o and pre_ml; and everything else on the warp-level products
 cudaError_t launch_attn_shared_umma(cudaStream_t s, int dtype, const SharedAttn& p);
 cudaError_t launch_attn_shared_rows(cudaStream_t s, const SharedAttn& p, uint32_t warps);  // float32, eight queries a warp

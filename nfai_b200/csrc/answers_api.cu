@@ -140,7 +140,7 @@ static const char* bad_attn_sizes(int dtype, uint32_t B, uint32_t qH, uint32_t k
 
 size_t nfai_op_attn_shared_scratch_bytes(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
   if (!B || bad_attn_sizes(dtype, B, qH, kvH, d, prefix, capacity)) return 0;
-  return plan_shared_attn(dtype, B, qH, kvH, d, prefix, capacity).total;
+  return shared_attn_scratch(dtype, B, qH, kvH, d, prefix, capacity);
 }
 
 int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const void* v_prefix, uint32_t prefix, const void* k_own,

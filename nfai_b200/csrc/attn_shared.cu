@@ -292,6 +292,12 @@ cudaError_t launch_own(cudaStream_t s, const SharedAttn& p, const SharedPlan& pl
 
 }  // namespace
 
+namespace {
+constexpr uint32_t kLeastOfAll = 32;                                                            // keys of a part of the own rows at least
+constexpr uint32_t own_rows_of(bool tensor, uint32_t G) { return tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8); }  // query heads of a CTA
+constexpr uint32_t own_ctas_of(bool tensor) { return 148 * (tensor ? 2 : 4); }                   // CTAs that the own rows are cut into
+}  // namespace
+
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
   SharedPlan a;
   const uint32_t G = qH / kvH;
@@ -323,13 +329,13 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
     a.pre_splits = (tiles + a.pre_tiles - 1) / a.pre_tiles;
   }
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
-  a.rows = a.tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8);
+  a.rows = own_rows_of(a.tensor, G);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
   // CTAs for every SM twice over (the CUDA cores' four times) where the keys go so far. A part has 128 keys at least where the walk of the
   // shared rows hides the time it takes (8 sequences behind 2011 rows: 11.4 us, 11.9 with 64, 12.3 with 32; 5 behind 100003: 46.3, 45.5,
   // 44.6), 32 where it is all there is (2 sequences of 340 keys and a join: 5.9 us, 6.2 with 64, 6.1 with 128).
-  a.own_least = !a.tensor ? 64 : shared ? 128 : 32;
-  uint64_t parts = (148 * (a.tensor ? 2 : 4) + groups - 1) / groups;
+  a.own_least = !a.tensor ? 64 : shared ? 128 : kLeastOfAll;
+  uint64_t parts = (own_ctas_of(a.tensor) + groups - 1) / groups;
   if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;
   if (parts > kMaxOwnSplits) parts = kMaxOwnSplits;
   // Up to 8 CTAs of a sequence's heads join their parts among each other, as a cluster, and where more are wanted for few keys it is 8: a
@@ -357,6 +363,26 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   a.own_o = take(a.joined ? a.own_splits * rows * d * 4 : 0);
   a.total = off > 256 ? off : 256;  // (one part per row needs none: a size is never 0)
   return a;
+}
+
+// A plan's scratch goes up and down with the sizes: more rows are cut into fewer parts. Of both kinds, rows times parts are bounded:
+//   shared rows   parts <= CTAs / (CTAs that have all rows once), and a CTA has 256 rows at most (float32: 16 warps an SM with 8 each);
+//   own rows      parts <= CTAs / (CTAs that have all rows once) + 1, and a CTA has own_rows_of rows;
+// and parts are no more than tiles of keys. Each bound grows with the batch, the prefix and the capacity.
+size_t shared_attn_scratch(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
+  const bool tensor = dtype != 0 && d <= 128;
+  const uint64_t G = qH / kvH, R = (uint64_t)B * G, rows = (uint64_t)B * qH;
+  auto least = [](uint64_t a, uint64_t b) { return a < b ? a : b; };
+  auto most = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+  uint64_t pre = 0;
+  if (tensor || dtype == 0) {
+    const uint64_t tile = tensor ? kPreTile : attn_shared_rows_keys(d), ctas_rows = tensor ? 148 * least(R, 2 * kPreRows) : 148 * 16 * 8;
+    pre = least(least((prefix + tile - 1) / tile, kMaxPreSplits) * rows, most(rows, ctas_rows));
+  }
+  const uint64_t keys = (uint64_t)capacity + prefix, own_rows = least(G, own_rows_of(tensor, (uint32_t)G));
+  const uint64_t own = least(least(most(1, (keys + kLeastOfAll - 1) / kLeastOfAll), kMaxOwnSplits) * rows, own_ctas_of(tensor) * own_rows + rows);
+  const uint64_t bytes = (pre + own) * (d + 2) * 4 + 4 * 255;  // sums, maxima and sums of weights, each on 256 bytes
+  return (bytes + 255) / 256 * 256;
 }
 
 cudaError_t launch_shared_attn(cudaStream_t s, int dtype, const SharedAttn& p, const SharedPlan& plan) {

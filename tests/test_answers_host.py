@@ -107,3 +107,40 @@ def test_frequencies_refused(args):
     with pytest.raises(_lib.NfaiError) as e:
         frequencies(*args)
     assert e.value.code == _lib.ERR_ARG
+
+
+def test_scratch_of_the_largest_step_serves_every_smaller_one():
+    """A host allocates once, for the largest batch, prompt and capacity that it will run; what a call needs (the text of a refusal says it) is
+    never more."""
+    need = _lib.load().nfai_op_attn_shared_scratch_bytes
+
+    def used(**sizes):
+        text = refusal("nfai_op_attn_shared", *{**ATTN, **sizes, "scratch_bytes": 0}.values())
+        assert "too small: 0 < " in text, text
+        return int(text.rsplit(" ", 1)[1])
+    batches = [1, 2, 3, 4, 5, 8, 15, 16, 17, 31, 32, 33, 37, 63, 64, 65, 74, 128, 129, 200, 256, 300, 600]
+    prefixes = [0, 1, 129, 300, 700, 1500, 2500, 3130, 4000, 9000, 20000, 32768, 100003]
+    capacities = [0, 1, 40, 64, 300, 512, 1024, 5000]
+    for dtype in (_lib.F32, _lib.F16):
+        for qH, kvH, d in ((32, 8, 64), (32, 8, 128), (16, 16, 64), (16, 1, 128), (6, 2, 32), (20, 1, 256), (48, 2, 80)):
+            sizes = dict(dtype=dtype, qH=qH, kvH=kvH, d=d)
+            before = {}
+            for B in batches:
+                for P in prefixes:
+                    for cap in capacities:
+                        n = need(dtype, B, qH, kvH, d, P, cap)
+                        assert n % 256 == 0 and n >= max(before.get((P, cap), 0), used(B=B, prefix=P, capacity=cap, **sizes)), (sizes, B, P, cap)
+                        before[P, cap] = n
+                for a, b in zip(prefixes, prefixes[1:]):
+                    assert all(before[a, cap] <= before[b, cap] for cap in capacities), (sizes, B, a, b)
+                for a, b in zip(capacities, capacities[1:]):
+                    assert all(before[P, a] <= before[P, b] for P in prefixes), (sizes, B, a, b)
+
+
+def test_scratch_is_not_far_above_what_a_step_uses():
+    """The bound goes by the most parts that any smaller step is cut into: at most so much per CTA of the GPU, or per row of the output."""
+    need = _lib.load().nfai_op_attn_shared_scratch_bytes
+    for dtype, B, qH, kvH, d, P, cap in ((_lib.F16, 64, 32, 8, 128, 32768, 1024), (_lib.F16, 256, 32, 8, 64, 1500, 2048), (_lib.F16, 2, 32, 8, 64, 300, 128),
+                                         (_lib.F32, 9, 8, 2, 32, 1000, 512), (_lib.BF16, 8, 32, 8, 128, 2011, 1024), (_lib.F16, 600, 32, 8, 128, 100003, 5000)):
+        # 148 CTAs with 256 rows each of the shared rows' parts, up to 592 with 16 of the own rows', and a row of each for every query head
+        assert need(dtype, B, qH, kvH, d, P, cap) <= (148 * 256 + 592 * 16 + 2 * B * qH) * (d + 2) * 4 + 1024
