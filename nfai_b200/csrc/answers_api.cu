@@ -156,7 +156,9 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
       return fail(c, NFAI_ERR_ARG, "pointers must be 16-byte aligned, scratch 256");
   }
   const SharedPlan plan = B ? plan_shared_attn(dtype, B, qH, kvH, d, prefix, capacity) : SharedPlan();
-  if (scratch_bytes < plan.total) return fail(c, NFAI_ERR_ARG, "scratch too small: %zu < %zu", scratch_bytes, plan.total);
+  // (as much as ..scratch_bytes says, which is never less than the plan's: what is refused follows from the sizes in a way that a host can use)
+  const size_t bound = B ? shared_attn_scratch(dtype, B, qH, kvH, d, prefix, capacity) : 0, need = plan.total > bound ? plan.total : bound;
+  if (scratch_bytes < need) return fail(c, NFAI_ERR_ARG, "scratch too small: %zu < %zu", scratch_bytes, need);
   ON_DEVICE(c);
   if (!B) return NFAI_OK;
   SharedAttn p;
