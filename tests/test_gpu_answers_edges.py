@@ -8,7 +8,7 @@ import pytest
 
 from nfai_b200 import build
 
-from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step
+from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step, rope_args, rope_call
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -124,3 +124,39 @@ def test_a_wait_that_gave_up_is_told_by_the_next_call_that_waits(tmp_path):
                     "-Wl,-rpath," + os.path.dirname(lib), "-L", os.path.join(cuda, "lib64"), "-lcudart_static", "-lpthread", "-ldl", "-lrt"], check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, (r.returncode, r.stdout, r.stderr)
+
+
+# ---- rotary rows: alignment ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("x,out", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f32"), ("f32", "f16"), ("f16", "f32")])
+def test_rope_rows_on_16_bytes(cuda_ctx, x, out, layout):
+    """Buffers that begin on an odd multiple of 16 bytes give the same bits as others, and take no kernel that goes an element at a time: that one
+    takes several times as long, here at most twice is allowed."""
+    names = ("x", "q", "k", "v")
+    even = rope_args(2011, 32, 8, 64, 64, layout, x, out, 2100, 7, slots="all")
+    odd = dict(even)
+    for n in names:
+        room = torch.empty(even[n].numel() + 16, device="cuda", dtype=even[n].dtype)
+        odd[n] = room[16 // room.element_size():][:even[n].numel()].view(even[n].shape)
+        odd[n].copy_(even[n])
+        assert odd[n].data_ptr() % 32 == 16 and even[n].data_ptr() % 32 == 0
+    stream = torch.cuda.Stream()
+    codes = TYPES[x][1], TYPES[out][1]
+
+    def timed(s):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(2_000_000)  # the calls are enqueued behind it, so that the host's time does not count
+            a.record()
+            for _ in range(20):
+                rope_call(cuda_ctx, s, *codes, stream=stream.cuda_stream)
+            b.record()
+        b.synchronize()
+        return a.elapsed_time(b)
+    torch.cuda.synchronize()
+    times = [(timed(even), timed(odd)) for _ in range(7)][2:]
+    for n in names:
+        assert torch.equal(even[n], odd[n])
+    even_ms, odd_ms = (sorted(t)[len(t) // 2] for t in zip(*times))
+    print(f"{x} {out} {layout}: {even_ms * 50:.2f} {odd_ms * 50:.2f} us")
+    assert odd_ms <= 2 * even_ms
