@@ -99,8 +99,9 @@ int nfai_tp_import_peers(nfai_ctx* ctx, const void* descs, int n);
 /* replaces: LlamaModelFactory.Dispose (LlamaModelFactory.cs:24-32). */
 int nfai_ctx_destroy(nfai_ctx* ctx);
 
-/* Budget, in nanoseconds, of every device-side wait on another rank (exchange words) and, where a decode step is one
- * resident kernel (nfai_step_kernels), of its CTAs' waits on one another. Default one second, or the environment
+/* Budget, in nanoseconds, of every device-side wait on another rank (exchange words), where a decode step is one
+ * resident kernel (nfai_step_kernels), of its CTAs' waits on one another, and of the waits for copies and products in
+ * nfai_op_attn_shared and nfai_op_logit_rules (at most 4 seconds). Default one second, or the environment
  * variable NFAI_WAIT_NS at context creation. A wait that runs out makes the call return NFAI_ERR_TIMEOUT; the kernel
  * itself always returns, and the cache row of that step is not valid (nfai_set_position goes back). Takes effect for
  * graphs captured afterwards (nfai_model_finalize, nfai_model_tune) and for the next resident step.
@@ -403,8 +404,8 @@ int nfai_op_sample_top_p(nfai_ctx* c, const float* logits, uint32_t V, float tem
  * `stream`: NULL runs on the context's own stream and returns when the result is there, as every nfai_op_* above. Otherwise it is a
  * cudaStream_t of the context's device (cudaStreamLegacy, the value 1, names the default stream): the work is put on that stream, the
  * call returns at once and may be captured into a graph; scratch and buffers must then not be used by work that may run at the same
- * time. The caller's current device stays what it was. Kernels that wait for copies or products give up after a while, leave NaN in
- * what they were to write, and note it: the next call without a stream to the attention or the rules returns NFAI_ERR_TIMEOUT then. */
+ * time. The caller's current device stays what it was. Kernels that wait for copies or products give up after the context's budget,
+ * leave NaN in what they were to write, and note it: the next call without a stream to the attention or the rules returns NFAI_ERR_TIMEOUT then. */
 
 enum { NFAI_ROPE_PAIRS = 0 /* elements 2i and 2i+1, the reference's layout */, NFAI_ROPE_HALVES = 1 /* i and i + dims/2 */ };
 enum { NFAI_ROPE_PLAIN = 0, NFAI_ROPE_LINEAR = 1, NFAI_ROPE_BANDS = 2, NFAI_ROPE_YARN = 3 };

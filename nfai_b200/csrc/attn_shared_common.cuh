@@ -26,17 +26,36 @@ __device__ __forceinline__ float s_ex2(float x) {
   return y;
 }
 
-// Bounded waits as in umma.cuh; the limit is counted in cycles, whose counter is read in a few of them (the nanosecond timer takes
-// longer than some of these waits).
-constexpr long long kWaitCycles = 2000000000ll;
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
-  if (umma::bar_try(bar, parity)) return true;
+// Bounded waits as in umma.cuh, with the context's budget; it is counted in cycles (two a nanosecond), whose counter is read in a few of
+// them (the nanosecond timer takes longer than some of these waits). How long one try may sleep is up to the hardware: with a budget below
+// a millisecond the barrier is asked without sleeping.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t ns) {
+  const bool sleep = ns >= 1000000u;
+  if (sleep && umma::bar_try(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!umma::bar_try(bar, parity))
-    if (clock64() - t0 > kWaitCycles) return false;
+  while (sleep ? !umma::bar_try(bar, parity) : !bar_test(bar, parity))
+    if (clock64() - t0 > 2ll * ns) return false;
   return true;
 }
-__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(bar, parity)); }
+// Where one gave up: a millisecond, for copies and products that are on their way to end before their memory is used for something else. (They
+// take some microseconds.)
+__device__ __forceinline__ void let_land() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 2000000ll) {
+  }
+}
+__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity, uint32_t ns) { return __all_sync(0xffffffffu, wait_for(bar, parity, ns)); }
 
 // The walk of one CTA: keys [t0, t1) of sequence b's n, the shared rows first unless they have kernels of their own.
 struct Walk {

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
     const uint32_t cnt = count_of(i);
     __syncwarp();  // every lane is past its reads of the stage that is filled next
     if (i + (NST - 1) * kMW < slices && ok) issue(i + (NST - 1) * kMW);
-    ok = __all_sync(0xffffffffu, ok && wait_for(full + 8 * use, phase));
+    ok = __all_sync(0xffffffffu, ok && wait_for(full + 8 * use, phase, p.wait_ns));
     const uint32_t ks = ring + use * 2 * SH::kHalf, vs = ks + SH::kHalf;
     if (cnt < kSlice) {
       unsigned char* const v = stages + (use * 2 + 1) * SH::kHalf;
@@ -230,9 +230,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
   }
   if (!ok) {
     if (lane == 0 && p.err) atomicOr(p.err, 4u);
-    // copies may still be on their way: a bounded time for them to end before their memory is used for something else
-    for (volatile uint32_t spin = 0; spin < (1u << 20); ++spin) {
-    }
+    let_land();
   }
   __syncthreads();  // every warp is past its last read of its stages: the warps' rows go where they were
   constexpr uint32_t PL = D + 4;

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     uint32_t j = 0;
     auto load = [&](const CUtensorMap* map, uint32_t it) {
       const uint32_t s = j % SM::kSlots;
-      if (j >= SM::kSlots && !all_wait_for(empty0 + 8 * s, (j / SM::kSlots - 1) & 1)) return ok = false;
+      if (j >= SM::kSlots && !all_wait_for(empty0 + 8 * s, (j / SM::kSlots - 1) & 1, p.wait_ns)) return ok = false;
       if (elect_one()) {
         bar_expect_tx(full0 + 8 * s, SM::kTile);
 #pragma unroll
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       for (uint32_t it = 0; it < n && ok; ++it)
         if (!load(&mapK, it) || !load(&mapV, it)) break;
     }
-    if (ok) ok = drain_ring<SM::kSlots>(empty0, j);
+    // the last slots' products, as drain_ring does, within the budget
+    for (uint32_t i = j > SM::kSlots ? j - SM::kSlots : 0; i < j && ok; ++i) ok = all_wait_for(empty0 + 8 * (i % SM::kSlots), i / SM::kSlots & 1, p.wait_ns);
   } else if (warp == 17) {
     // 16-bit operands, float32 sums; A along K in both products; B along K (K tile) or along N (V tile)
     constexpr uint32_t idesc_s = kTypes | ((kPreTile >> 3) << 17) | ((kPreRows >> 4) << 24);
@@ -221,12 +222,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         umma_commit(s_ready(u));
       }
     };
-    ok = all_wait_for(q_ready, 0);  // Q, and the first keys' tiles
+    ok = all_wait_for(q_ready, 0, p.wait_ns);  // Q, and the first keys' tiles
     fence_after();
     for (uint32_t u = 0; u < NB && u < units && ok; ++u) scores(u);
     for (uint32_t u = 0; u < units && ok; ++u) {
       const uint32_t st = u & 1, it = u >> 1, j = values_of(u);  // it: the stream's own count
-      if (!(ok = all_wait_for(p_ready(u), p_turn(u)))) break;  // the weights, the values' tile and the next scores' keys
+      if (!(ok = all_wait_for(p_ready(u), p_turn(u), p.wait_ns))) break;  // the weights, the values' tile and the next scores' keys
       fence_after();
       if (elect_one()) {
         const uint32_t s = j % SM::kSlots, v_s = base + SM::kRing + s * SM::kTile;
@@ -245,13 +246,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     const uint32_t tiles = 2 * n;
     uint32_t seen = 0;
     auto see = [&](uint32_t upto) {  // the first `upto` tiles have arrived
-      for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1);
+      for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1, p.wait_ns);
     };
     see(min(tiles, twice ? NB : (NB - 1) / 2 * 2 + 1));
     if (ok && lane == 0) bar_arrive(q_ready);
     for (uint32_t u = 0; u < units && ok; ++u) {
       see(min(tiles, twice ? 2 * u + NB + 2 : (u + NB) / 2 * 2 + 1));
-      if (u >= NB && ok) ok = all_wait_for(p_ready(u), p_turn(u - NB));  // (the phase before has ended: this arrival is for the next)
+      if (u >= NB && ok) ok = all_wait_for(p_ready(u), p_turn(u - NB), p.wait_ns);  // (the phase before has ended: this arrival is for the next)
       if (ok && lane == 0) bar_arrive(p_ready(u));
     }
   } else {
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       // These scores are there, and the products that were issued before them are done: with NB = 2 that of this stream's last tile is
       // one of them, with NB = 3 that of the tile before. (A warp that gave up still meets the other one.)
       const uint32_t u = 2 * it + st, cS = u % NB * kSP;
-      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(u), s_turn(u)));
+      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(u), s_turn(u), p.wait_ns));
       if (!there) {
         __syncwarp();
         if (lane == 0) bar_arrive(p_ready(u));
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           if (it) {
             const float f = p_ex2(before - ref);
             l *= f;
-            if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1));
+            if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1, p.wait_ns));
             fence_after();
 #pragma unroll 1
             for (uint32_t k = half * (D / 2); k < (half + 1) * (D / 2); k += 16) {
@@ -393,16 +394,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       __syncwarp();
       if (lane == 0) bar_arrive(p_ready(u));
     }
-    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_last(st), 0));
+    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_last(st), 0, p.wait_ns));
     if (there) {
       swap[half * kPreRows + place] = l;
       meet();
       l += swap[(half ^ 1) * kPreRows + place];
     }
-    // Every score -infinity: as if there were no keys. A wait that gave up: NaN.
+    // Every score -infinity: as if there were no keys.
     float2 ml = make_float2(ref, l);
     if (m <= floor && l < 0.5f) ml = make_float2(-INFINITY, 0.f);
-    if (!ok) ml = make_float2(0.f, __uint_as_float(0x7fffffffu));
     // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
     // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,
     // eight by eight in an order that follows from the row: no bank is met twice.
@@ -463,18 +463,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       }
     }
   }
-  if (!ok) {
-    if (lane == 0 && p.err) atomicOr(p.err, 4u);
-    // copies and products of this CTA may still be in flight: a bounded time for them to end before their memory is released
-    for (volatile uint32_t spin = 0; spin < (1u << 20); ++spin) {
-    }
-  }
   fence_before();
-  const bool mend = __syncthreads_or(odd != odd);
+  const uint32_t r0 = tile * kPreRows, r1 = min(R, r0 + 2 * kPreRows);
+  const bool mend = __syncthreads_or(odd != odd || !ok);
+  // A warp that gave up has arrived where it had not worked, for its own rows and those of others: no row of the CTA is a number then.
+  if (mend && __syncthreads_or(!ok)) {
+    if (tid == 0 && p.err) atomicOr(p.err, 4u);
+    for (uint32_t r = r0 + tid; r < r1; r += kThreads)
+      *reinterpret_cast<float2*>(p.pre_ml + (((uint64_t)split * p.kvH + g) * R + r) * 2) = make_float2(0.f, __uint_as_float(0x7fffffffu));
+    shared_attn::let_land();  // nobody issues copies or products any more, but some may be in flight
+    __syncthreads();
+  } else if (mend) {
+    shared_attn::mend_shared<T>(p, split, g, r0, r1, first * kPreTile, min(p.prefix, (first + n) * kPreTile), warp, kThreads / 32);
+  }
   if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  if (mend)
-    shared_attn::mend_shared<T>(p, split, g, tile * kPreRows, min(R, (tile + 2) * kPreRows), first * kPreTile, min(p.prefix, (first + n) * kPreTile), warp,
-                                kThreads / 32);
 }
 
 template <typename T, int D, int COPIES>

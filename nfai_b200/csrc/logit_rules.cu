@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     if (t < len) atomicAdd(count + t, 1u);
   }
   if (front && peel) in_front([&](uint32_t c, uint32_t) { atomicAdd(count + c, 1u); });
-  const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0));  // the slice is there, and everything is counted
+  const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0, p.wait_ns));  // the slice is there, and everything is counted
   if (n_hist) {
     auto rule = [&](uint32_t c, uint32_t t) {  // whoever finds a count takes it and leaves none
       const uint32_t n = atomicExch(count + c, 0u);
@@ -183,9 +183,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
   if (front && tid < peel && !open(tid)) value[S + tid] = -INFINITY;
   if (!ok) {
     if (p.err && tid == 0) atomicOr(p.err, 4u);
-    // the copy may still be on its way: a bounded time for it to end before its memory is used for something else
-    for (volatile uint32_t spin = 0; spin < (1u << 20); ++spin) {
-    }
+    shared_attn::let_land();
     __syncthreads();
     for (uint32_t i = tid; i < whole; i += kLT) value[i] = __int_as_float(0x7fffffff);
   }

@@ -1,14 +1,14 @@
-"""Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest, infinite values. The helpers and the
-conventions on tolerances are those of test_gpu_answers.py."""
+"""Where the operators of a step of several answers to one prompt could go wrong: weights far below a row's heaviest, infinite values,
+alignment, waits that run out. The helpers and the conventions on tolerances are those of test_gpu_answers.py."""
 import os
 import shutil
 import subprocess
 
 import pytest
 
-from nfai_b200 import build
+from nfai_b200 import _lib, build
 
-from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step, rope_args, rope_call
+from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step, rope_args, rope_call, run
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -160,3 +160,62 @@ def test_rope_rows_on_16_bytes(cuda_ctx, x, out, layout):
     even_ms, odd_ms = (sorted(t)[len(t) // 2] for t in zip(*times))
     print(f"{x} {out} {layout}: {even_ms * 50:.2f} {odd_ms * 50:.2f} us")
     assert odd_ms <= 2 * even_ms
+
+
+@pytest.mark.parametrize("B,kvH,G,d,P,cap,kind", [(24, 8, 4, 64, 1500, 40, "f16"), (24, 8, 4, 128, 1500, 40, "bf16"), (9, 2, 3, 128, 6000, 300, "f16"), (70, 8, 8, 64, 2500, 60, "bf16"),
+                                                  (40, 8, 4, 64, 100, 2000, "f16"), (300, 2, 2, 32, 90, 900, "bf16"), (200, 8, 4, 64, 1500, 60, "f16")])
+def test_a_wait_that_runs_out_leaves_no_number(cuda_ctx, B, kvH, G, d, P, cap, kind):
+    """With a budget of a nanosecond the kernels give up on their copies: they return, the call says so, and what a row then has is NaN, or, where
+    nothing had to be waited for, what it has otherwise. Nothing is left for the next call."""
+    def budget(ns):
+        _lib.check(_lib.load().nfai_ctx_set_wait_ns(cuda_ctx.handle, ns), cuda_ctx.handle)
+    s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d)
+    attn_call(cuda_ctx, s)
+    want = s["out"].clone()
+
+    def nan_or_right():
+        heads, right = s["out"].view(-1, d), want.view(-1, d)
+        gone = heads.isnan().all(-1)
+        assert torch.equal(heads[~gone], right[~gone])
+        return gone.float().mean().item()
+    try:
+        budget(1)
+        for _ in range(3):
+            s["out"].fill_(5.0)
+            with pytest.raises(_lib.NfaiError) as e:
+                attn_call(cuda_ctx, s)
+            assert e.value.code == _lib.ERR_TIMEOUT
+            assert nan_or_right() > 0
+        attn_call(cuda_ctx, s, stream=torch.cuda.current_stream().cuda_stream or 1)  # on a stream nobody is told yet
+        torch.cuda.synchronize()
+        assert nan_or_right() > 0
+    finally:
+        budget(1_000_000_000)
+    with pytest.raises(_lib.NfaiError) as e:  # the next call that waits is, and is right itself
+        attn_call(cuda_ctx, s)
+    assert e.value.code == _lib.ERR_TIMEOUT and torch.equal(s["out"], want)
+    s["out"].fill_(5.0)
+    attn_call(cuda_ctx, s)
+    assert torch.equal(s["out"], want)
+
+
+def test_a_wait_that_runs_out_in_the_rules(cuda_ctx):
+    def budget(ns):
+        _lib.check(_lib.load().nfai_ctx_set_wait_ns(cuda_ctx.handle, ns), cuda_ctx.handle)
+    x = torch.randn(700, 100000, device="cuda")  # more than the L2 holds
+    out = torch.empty_like(x)
+
+    def call():  # (nothing is asked for: there is nothing to do while the logits come)
+        out.fill_(5.0)
+        run(cuda_ctx, "nfai_op_logit_rules", x.data_ptr(), 700, 100000, *[None, 0] + [None] * 7, 0, None, 0, None, out.data_ptr())
+    try:
+        budget(1)
+        with pytest.raises(_lib.NfaiError) as e:
+            call()
+        assert e.value.code == _lib.ERR_TIMEOUT
+        gone = out.isnan()
+        assert gone.any() and torch.equal(out[~gone], x[~gone])
+    finally:
+        budget(1_000_000_000)
+    call()
+    assert torch.equal(out, x)
