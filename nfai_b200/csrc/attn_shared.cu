@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kST) attn_shared_any_kernel(const __grid_const
     float a = 0.f;
     for (uint32_t k = 0; k < KG; ++k) a += K[(r * KG + k) * d + e];
     q[i] = a;  // (the queries have been used)
-    odd |= a != a;
+    odd |= a != a && is_sum(l[r]);
   }
   if (__syncthreads_or(odd)) {
     mend_part<T, kST>(p, b, h0, nh, walk.t0, walk.t1, q, d, l);

@@ -91,7 +91,8 @@ __device__ __forceinline__ uint64_t key_row(const SharedAttn& p, uint32_t b, uin
 // A sum of weighted values comes out as no number where an infinite value meets a weight, or a term of one, that is 0 in the type of the
 // product: the second term of a weight that is exact, a key that belongs to another copy of the row, a weight that is too small for float16.
 // Weights are above 0, so infinities of one sign are the sum, and those of both signs or a NaN are none. Which it is follows from the column of
-// values alone; the kernels look at it again, for the keys of their part, where a row whose weights' sum is a number has such an element.
+// values alone; the kernels look at it again, for the keys of their part, where a row whose weights' sum is a number has such an element. (Only
+// there: a free place of the batch may hold queries that are no numbers.)
 // `acc` becomes NaN where one of the four is
 __device__ __forceinline__ void note_nan(float& acc, float4 v) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(acc) : "f"(v.x));

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
       }
     }
     *reinterpret_cast<float4*>(rows + j * PL + e) = acc;
-    note_nan(odd, acc);
+    if (is_sum(sum)) note_nan(odd, acc);
     if (e == 0) {
       M[j] = top;
       L[j] = sum;

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256) attn_shared_rows_kernel(const __grid_cons
       unpair(o[r][c][0], y.x, y.y);
       unpair(o[r][c][1], y.z, y.w);
       *reinterpret_cast<float4*>(p.pre_o + at * d + e) = y;
-      note_nan(odd, y);
+      if (is_sum(l[r])) note_nan(odd, y);
     }
     if (kg == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(m[r], l[r]);
   }

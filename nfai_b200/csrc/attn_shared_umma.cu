@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
   pdl_launch_dependents();  // the own rows do not wait for the shared ones, only the join does
   const uint32_t units = twice ? n : 2 * n;  // unit u: stream u % 2, tile of keys u or u / 2
   bool ok = true;
-  float odd = 0.f;  // NaN: one is among the sums that this thread has written
+  float odd = 0.f;  // NaN: one is among the sums of this thread's row
 
   if (warp == 16) {
     if (whole_q && elect_one()) {
@@ -417,10 +417,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         uint32_t o[32];
         tmem_ld(lanes + cO + half * (D / 2) + k * 4, o);
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e)
-          *reinterpret_cast<uint4*>(sums + piece(place, half * (kPieces / 2) + k + e)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        for (uint32_t e = 0; e < 8; ++e) {
+          const float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          *reinterpret_cast<float4*>(sums + piece(place, half * (kPieces / 2) + k + e)) = v;
+          shared_attn::note_nan(odd, v);
+        }
       }
     }
+    if (!shared_attn::is_sum(ml.y)) odd = 0.f;
     if (twice) {
       if (half == 0) {
         swap[place] = ml.x;
@@ -447,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         }
         const uint64_t at = ((uint64_t)split * p.kvH + g) * R + r;
         if (e * 4 < d) *reinterpret_cast<float4*>(p.pre_o + at * d + e * 4) = acc;
-        shared_attn::note_nan(odd, acc);
         if (e == 0) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(top, total);
       }
     } else if (there) {
@@ -459,7 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         const uint32_t r = i / (kPieces / 2), e = half * (kPieces / 2) + i % (kPieces / 2);
         const float4 v = *reinterpret_cast<const float4*>(sums + piece(quarter * 32 + r, e));
         if (row - lane + r < R && e * 4 < d) *reinterpret_cast<float4*>(p.pre_o + (at0 + row - lane + r) * d + e * 4) = v;
-        shared_attn::note_nan(odd, v);
       }
     }
   }
