@@ -44,7 +44,7 @@ bool known_dtype(int t) { return t == NFAI_F32 || t == NFAI_F16 || t == NFAI_BF1
   OnDevice on_device((c)->device);                          \
   if (on_device.err != cudaSuccess) return fail((c), NFAI_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(on_device.err))
 
-constexpr double kPi = 3.14159265358979323846;
+constexpr double kPi = 3.14159265358979323846, kLog2e = 1.4426950408889634;
 
 }  // namespace
 
@@ -148,7 +148,7 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
                         const void* v_own, uint32_t capacity, const int32_t* lens, int dtype, uint32_t B, uint32_t qH, uint32_t kvH,
                         uint32_t d, float scale, void* out, void* scratch, size_t scratch_bytes, void* stream) {
   if (const char* wrong = bad_attn_sizes(dtype, B, qH, kvH, d, prefix, capacity)) return fail(c, NFAI_ERR_ARG, "%s", wrong);
-  if (!(scale >= 0.f) || scale > FLT_MAX) return fail(c, NFAI_ERR_ARG, "scale must be positive, or 0 for 1 / sqrt(d)");
+  if (!(scale >= 0.f) || scale * kLog2e > FLT_MAX) return fail(c, NFAI_ERR_ARG, "scale must be positive, or 0 for 1 / sqrt(d), and below 2^127.4");
   if (B) {
     if (!q || !out || !lens || !scratch || (prefix && (!k_prefix || !v_prefix)) || (capacity && (!k_own || !v_own)))
       return fail(c, NFAI_ERR_ARG, "null argument");
@@ -166,7 +166,7 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   char* const base = static_cast<char*>(scratch);
   p.q = q; p.kp = k_prefix; p.vp = v_prefix; p.ko = k_own; p.vo = v_own; p.lens = lens; p.prefix = prefix; p.capacity = capacity;
   p.B = B; p.qH = qH; p.kvH = kvH; p.d = d; p.out = out;
-  p.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)d)) * 1.4426950408889634);
+  p.scale2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)d)) * kLog2e);
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
   p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
   p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined;

@@ -144,3 +144,10 @@ def test_scratch_is_not_far_above_what_a_step_uses():
                                          (_lib.F32, 9, 8, 2, 32, 1000, 512), (_lib.BF16, 8, 32, 8, 128, 2011, 1024), (_lib.F16, 600, 32, 8, 128, 100003, 5000)):
         # 148 CTAs with 256 rows each of the shared rows' parts, up to 592 with 16 of the own rows', and a row of each for every query head
         assert need(dtype, B, qH, kvH, d, P, cap) <= (148 * 256 + 592 * 16 + 2 * B * qH) * (d + 2) * 4 + 1024
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 2.4e38])
+def test_a_scale_that_leaves_float32_is_refused(scale):
+    """The kernels use scale * log2(e)."""
+    assert "scale" in refusal("nfai_op_attn_shared", *{**ATTN, "scale": scale}.values())
+    assert "ctx is null" in refusal("nfai_op_attn_shared", *{**ATTN, "scale": 2.3e38}.values())
