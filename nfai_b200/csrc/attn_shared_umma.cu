@@ -42,6 +42,7 @@ using shared_attn::wait_for;
 
 constexpr int kSoftmax = 512, kThreads = kSoftmax + 96;
 constexpr float kGrowth = 8.0f;
+constexpr float kFar = 1048576.0f;  // 2^20: from here on a ref is off by 2^-3 and more
 // Weights are multiplied by 2^kLift before they are rounded (the weights' sum has the factor too, and the maximum that goes to scratch is
 // lower by it). float16 ends at 2^-25: without the factor a key that is 2^-25 lighter than its row's heaviest counts for nothing, and 100 000 of
 // them behind a heavy one are 0.003 of the row. 2^(kGrowth + kLift) is within float16, whose largest number is 2^16. (2^4 and 2^11 rescale more
@@ -291,10 +292,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           : "memory");
       return r != 0;
     };
-    // m: the maximum that counts, of the scores as they are; ref: what their exponents are taken from. Both this and the limit on growth are
-    // rounded such that no weight is above 2^(kGrowth + kLift), however large the scores.
+    // m: the maximum that counts, of the scores as they are; ref: what their exponents are taken from, an addend of the multiply-add. Both this
+    // and the limit on growth are rounded such that no weight is above 2^(kGrowth + kLift). far: the row's ref is so large that its last bit
+    // counts; the maximum is then taken from the scores before they are multiplied, and ref is what is left. (Row by row: a row of no numbers
+    // has a ref of this kind, and its neighbours keep their bits.)
     auto ref_of = [&](float top) { return __fadd_ru(__fmul_ru(top, c), -kLift<T>); };
     float m = floor, ref = 0.f, l = 0.f;
+    bool far = false, any_far = false;
     for (uint32_t it = 0; it < tiles; ++it) {
       // These scores are there, and the products that were issued before them are done: with NB = 2 that of this stream's last tile is
       // one of them, with NB = 3 that of the tile before. (A warp that gave up still meets the other one.)
@@ -332,9 +336,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           meet();
           top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + place]), m);
           const float before = ref;
+          const bool was_far = far;
           ref = ref_of(top);
+          far = fabsf(ref) > kFar;
+          any_far = __any_sync(0xffffffffu, far);
+          if (far) ref = -kLift<T>;
           if (it) {
-            const float f = p_ex2(before - ref);
+            const float f = p_ex2(far || was_far ? (m - top) * c : before - ref);
             l *= f;
             if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1, p.wait_ns));
             fence_after();
@@ -350,6 +358,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           m = top;
         }
         sum[0] = sum[1] = 0;
+        if (any_far) {
+          const float less = far ? m : 0.f;
+#pragma unroll
+          for (uint32_t j = 0; j < kMine; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) - less);
+        }
         const uint64_t minus_ref = pair(-ref, -ref);
         auto weights = [&](uint32_t k, uint32_t (&w)[kPart]) {
 #pragma unroll
@@ -401,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       l += swap[(half ^ 1) * kPreRows + place];
     }
     // Every score -infinity: as if there were no keys.
-    float2 ml = make_float2(ref, l);
+    float2 ml = make_float2(far ? ref_of(m) : ref, l);
     if (m <= floor && l < 0.5f) ml = make_float2(-INFINITY, 0.f);
     // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
     // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,

@@ -146,8 +146,7 @@ def test_a_wait_that_gave_up_is_told_by_the_next_call_that_waits(tmp_path):
 
 @pytest.mark.parametrize("d,P,kind", [(128, 8000, "bf16"), (64, 1500, "f16"), (64, 600, "f32")])
 def test_attention_queries_of_free_places_may_be_anything(cuda_ctx, d, P, kind):
-    """They are not looked at: neither the other rows' bits nor the time (60 % and more where sums that are no numbers were looked into for
-    them) depend on what they hold."""
+    """Where they are no numbers, the other rows' bits stay, and so does the time (60 % and more were lost where their sums were looked into)."""
     B = 64
     s = attn_args(kind, B, 32, 8, d, P, 40, [-1 if b % 20 == 7 else b % 41 for b in range(B)], seed=d)
     other = dict(s, q=s["q"].clone(), out=s["out"].clone())
@@ -237,3 +236,27 @@ def test_a_wait_that_runs_out_in_the_rules(cuda_ctx):
         budget(1_000_000_000)
     call()
     assert torch.equal(out, x)
+
+
+# ---- attention: scores of any size ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,spread", [("f16", 3e3), ("bf16", 1e5), ("bf16", 1e7), ("bf16", 1e9), ("bf16", 1e12), ("f32", 1e8), ("f32", 1e13)])
+@pytest.mark.parametrize("B,kvH,G,d,P,cap", [(2, 8, 4, 64, 300, 60), (5, 8, 4, 64, 9000, 100), (24, 8, 4, 128, 1500, 40), (70, 2, 8, 40, 2500, 60), (200, 8, 4, 64, 1500, 30)])
+def test_attention_scores_far_beyond_their_differences(cuda_ctx, kind, spread, B, kvH, G, d, P, cap):
+    """Scores so large that float32 leaves few bits or none behind the point: the largest has all the weight, whatever its size. Rows whose two
+    largest are nearer than float32 sums can tell (4 d u of the products' size) are left out; most remain. The result is a value of the cache: off
+    by half a step where the one weight is rounded and its sum is not, by 4 u for quotient and product, and by half a step of the result."""
+    s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d, spread=spread)
+    attn_call(cuda_ctx, s)
+    seen = 0
+    for b, n in enumerate(s["lens"].tolist()):
+        k = torch.cat([s["kp"].double(), s["ko"][b, :n].double()]).view(-1, kvH, d).permute(1, 2, 0)
+        v = torch.cat([s["vp"], s["vo"][b, :n]]).view(-1, kvH, d).permute(1, 0, 2)
+        q = s["q"][b].double().view(kvH, G, d)
+        best = (q @ k).topk(2, -1)
+        room = 4 * d * U * (q.abs() @ k.abs()).amax(-1) + 200 * d ** 0.5  # (and a weight of e^-200 is 0 in float32)
+        clear = best.values[..., 0] - best.values[..., 1] > room
+        want = v.gather(1, best.indices[..., :1].expand(-1, -1, d))
+        off = (s["out"][b].view(kvH, G, d).double() - want.double()).abs() / want.double().abs()
+        assert off[clear].max().item() <= 2 * half_step(TYPES[kind][0]) + 4 * U, b
+        seen += clear.float().mean().item()
+    assert seen > 0.5 * B
