@@ -26,6 +26,8 @@
 // 1.05 to 1.4 times as far from the one in 64 bits as with weights of 32, where the rounding of the result is nearly all.
 // Scores are products of the 16-bit queries as they are; the scale goes into the exponent's multiply-add. A row's sums are rescaled only
 // when its maximum has grown by more than 2^8 since the last time.
+#include <float.h>
+
 #include <type_traits>
 
 #include "attn_shared_common.cuh"
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     const uint32_t lanes = tmem + (quarter * 32u << 16), cO = kO + st * D;
     const uint32_t tiles = twice ? (n + 1 - st) / 2 : n;  // of this stream
     const bool there = __any_sync(0xffffffffu, row < R);  // else this warp's exponentials are left out
-    const float c = p.scale2, growth = __fdiv_rd(kGrowth, c), floor = c > 1.f ? -1e38f / c : -1e38f;
+    const float c = p.scale2, growth = __fdiv_rd(kGrowth, c), floor = c > 1.f ? __fdiv_rz(-FLT_MAX, c) : -FLT_MAX;
     const uint64_t c2 = pair(c, c);
     float* const swap = reinterpret_cast<float*>(sm + SM::kSwapOff) + st * 2 * kPreRows;  // [half][place]
     auto meet = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(st * 4 + quarter + 1) : "memory"); };
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     // and the limit on growth are rounded such that no weight is above 2^(kGrowth + kLift). far: the row's ref is so large that its last bit
     // counts; the maximum is then taken from the scores before they are multiplied, and ref is what is left. (Row by row: a row of no numbers
     // has a ref of this kind, and its neighbours keep their bits.)
-    auto ref_of = [&](float top) { return __fadd_ru(__fmul_ru(top, c), -kLift<T>); };
+    // floor: the lowest score that times c is a number, so that every such score counts.
     float m = floor, ref = 0.f, l = 0.f;
     bool far = false, any_far = false;
     for (uint32_t it = 0; it < tiles; ++it) {
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           top = fmaxf(fmaxf(top, swap[(half ^ 1) * kPreRows + place]), m);
           const float before = ref;
           const bool was_far = far;
-          ref = ref_of(top);
+          ref = __fadd_ru(__fmul_ru(top, c), -kLift<T>);
           far = fabsf(ref) > kFar;
           any_far = __any_sync(0xffffffffu, far);
           if (far) ref = -kLift<T>;
@@ -414,7 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       l += swap[(half ^ 1) * kPreRows + place];
     }
     // Every score -infinity: as if there were no keys.
-    float2 ml = make_float2(far ? ref_of(m) : ref, l);
+    // (What a part hands on is rounded as the kernel for the own rows rounds: equal scores stay equal there, however large.)
+    float2 ml = make_float2(far ? __fadd_ru(__fmul_rn(m, c), -kLift<T>) : ref, l);
     if (m <= floor && l < 0.5f) ml = make_float2(-INFINITY, 0.f);
     // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
     // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,

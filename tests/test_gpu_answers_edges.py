@@ -260,3 +260,28 @@ def test_attention_scores_far_beyond_their_differences(cuda_ctx, kind, spread, B
         assert off[clear].max().item() <= 2 * half_step(TYPES[kind][0]) + 4 * U, b
         seen += clear.float().mean().item()
     assert seen > 0.5 * B
+
+
+@pytest.mark.parametrize("B,kvH,G,d,P,cap", [(2, 8, 4, 64, 300, 60), (5, 8, 4, 64, 9000, 100), (24, 8, 4, 128, 1500, 40), (70, 2, 8, 40, 2500, 60), (200, 8, 4, 64, 1500, 30), (3, 2, 2, 256, 700, 9)])
+@pytest.mark.parametrize("kind,low", [("bf16", -3.3895313892515355e38), ("f32", -3.4028234663852886e38), ("f16", -65504.0)])
+def test_attention_rows_with_nothing_but_the_lowest_scores(cuda_ctx, kind, low, B, kvH, G, d, P, cap):
+    """Keys whose scores are the lowest number that the type has, as a mask leaves them (the query picks one element): where a row has nothing else
+    they weigh the same, and where it has others they weigh nothing."""
+    s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d)
+    s["q"].zero_()
+    s["q"].view(B, kvH, G, d)[..., 3] = 1.0
+    for k, v in ((s["kp"], s["vp"]), (s["ko"], s["vo"])):
+        k.view(*k.shape[:-1], kvH, d)[..., 3] = low
+        v.copy_(v.float().abs().clamp(0.25, 4.0))
+    # the last KV head has a few keys with scores of their own
+    s["kp"].view(P, kvH, d)[P // 3:P // 3 + 5, -1, 3] = 1.5
+    s["ko"].view(B, cap, kvH, d)[:, 1, -1, 3] = 1.5
+    for b, n in enumerate(s["lens"].tolist()):
+        s["ko"][b, n:], s["vo"][b, n:] = float("nan"), float("inf")
+    attn_call(cuda_ctx, s, scale=0.125)
+    want, size, _ = attn_want(s, scale=0.125)
+    half = half_step(TYPES[kind][0])
+    # equal scores, so equal weights: sums of n of them n u, quotient and product 4 u, weights in two terms 2^-16, the result half a step
+    room = ((P + cap + 8) * U + (2.0 ** -16 if kind != "f32" else 0.0) + half) * size
+    off = (s["out"].view(want.shape).double() - want).abs()
+    assert (off <= room).all(), (off / room).max().item()
