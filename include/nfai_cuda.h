@@ -458,7 +458,8 @@ size_t nfai_op_attn_shared_scratch_bytes(int dtype, uint32_t B, uint32_t qH, uin
  *   + the row's bias for the token: entries bias_start[row] .. bias_start[row+1]-1 of (bias_ids, bias); the last of several counts
  *   -infinity where bit (token % 32) of word token / 32 of mask mask_rows[row] is 0; masks is [n_masks][(V + 31) / 32]; a row
  *   whose mask_rows is not in 0 .. n_masks-1 (-1) is free; mask_rows null: row r has mask r
- * All device memory. history rows are history_stride apart, history_len null means all of it, tokens of V and above count for nothing.
+ * All device memory. history rows are history_stride apart, history_len null means all of it (and more than history_stride counts as that),
+ * tokens of V and above count for nothing; the last row's history may end with its tokens.
  * Null: history (no penalties), repetition (1), frequency and presence (0); n_bias = 0 and n_masks = 0: none. */
 int nfai_op_logit_rules(nfai_ctx* ctx, const float* logits, uint32_t rows, uint32_t V, const uint32_t* history, uint32_t history_stride,
                         const int32_t* history_len, const float* repetition, const float* frequency, const float* presence,

@@ -64,14 +64,19 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
                    : "memory");
     }
   }
-  // What decides what else is read comes first. A row's history has history_stride places whatever its length: the first are asked for too.
+  // What decides what else is read comes first. A row's history has history_stride places whatever its length, behind which the next row's
+  // begin: the first are asked for too. Behind the last row's tokens there need be no memory.
   const uint32_t* const h = p.history + (uint64_t)row * p.history_stride;
   const int32_t hist_len = p.history && p.history_len ? __ldg(p.history_len + row) : 0x7fffffff;
   const int32_t bias_lo = p.n_bias ? __ldg(p.bias_start + row) : 0, bias_hi = p.n_bias ? __ldg(p.bias_start + row + 1) : 0;
   const int64_t mrow = p.n_masks ? (p.mask_rows ? (int64_t)__ldg(p.mask_rows + row) : (int64_t)row) : -1;
   uint32_t seen[kSeen];
+  auto ask = [&](uint32_t places) {
 #pragma unroll
-  for (uint32_t k = 0; k < kSeen; ++k) seen[k] = p.history && tid + k * kLT < p.history_stride ? __ldg(h + tid + k * kLT) : 0xffffffffu;
+    for (uint32_t k = 0; k < kSeen; ++k) seen[k] = tid + k * kLT < places ? __ldg(h + tid + k * kLT) : 0xffffffffu;
+  };
+  if (!p.history || row + 1 < p.rows) ask(p.history ? p.history_stride : 0u);
+  else ask((uint32_t)min((int64_t)max(hist_len, 0), (int64_t)p.history_stride));
   const float rep = p.repetition ? __ldg(p.repetition + row) : 1.f, freq = p.frequency ? __ldg(p.frequency + row) : 0.f,
               pres = p.presence ? __ldg(p.presence + row) : 0.f;
   // what does not go 16 bytes at a time: the end of the slice, and tokens in front

@@ -8,7 +8,7 @@ import pytest
 
 from nfai_b200 import _lib, build
 
-from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step, rope_args, rope_call, run
+from .test_gpu_answers import TYPES, U, attn_args, attn_call, half_step, rope_args, rope_call, rules_args, rules_call, rules_check, rules_dev, run
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -285,3 +285,17 @@ def test_attention_rows_with_nothing_but_the_lowest_scores(cuda_ctx, kind, low, 
     room = ((P + cap + 8) * U + (2.0 ** -16 if kind != "f32" else 0.0) + half) * size
     off = (s["out"].view(want.shape).double() - want).abs()
     assert (off <= room).all(), (off / room).max().item()
+
+
+# ---- rules: the end of the history --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,V,H", [(1, 5000, 4000), (3, 128256, 3000), (40, 1000, 9000)])
+def test_rules_history_that_ends_with_the_last_rows_tokens(cuda_ctx, rows, V, H):
+    """Nothing behind them is read: what lies there here would count, and need not be there."""
+    s = rules_args(rows, V, H, 5, 0, seed=rows)
+    s["history_len"][:] = H
+    s["history_len"][-1] = 7
+    dev = rules_dev(s)
+    flat = torch.zeros(rows * H, device="cuda", dtype=torch.int32)  # token 0 behind them
+    flat[:(rows - 1) * H + 7] = dev["history"].reshape(-1)[:(rows - 1) * H + 7]
+    dev["history"] = flat
+    rules_check(s, rules_call(cuda_ctx, s, dev))
