@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     };
     // m: the maximum that counts, of the scores as they are; ref: what their exponents are taken from, an addend of the multiply-add. Both this
     // and the limit on growth are rounded such that no weight is above 2^(kGrowth + kLift). far: the row's ref is so large that its last bit
-    // counts; the maximum is then taken from the scores before they are multiplied, and ref is what is left. (Row by row: a row of no numbers
+    // counts; the maximum is then taken from the scores before they are multiplied. (Row by row: a row of no numbers
     // has a ref of this kind, and its neighbours keep their bits.)
     // floor: the lowest score that times c is a number, so that every such score counts.
     float m = floor, ref = 0.f, l = 0.f;
@@ -342,9 +342,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           ref = __fadd_ru(__fmul_ru(top, c), -kLift<T>);
           far = fabsf(ref) > kFar;
           any_far = __any_sync(0xffffffffu, far);
-          if (far) ref = -kLift<T>;
+          if (far) ref = 0.f;  // (and no lift: what a part hands on could not be lower by it)
           if (it) {
-            const float f = p_ex2(far || was_far ? (m - top) * c : before - ref);
+            const float lifted = far == was_far ? 0.f : far ? -kLift<T> : kLift<T>;
+            const float f = p_ex2(far || was_far ? (m - top) * c + lifted : before - ref);
             l *= f;
             if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1, p.wait_ns));
             fence_after();
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     }
     // Every score -infinity: as if there were no keys.
     // (What a part hands on is rounded as the kernel for the own rows rounds: equal scores stay equal there, however large.)
-    float2 ml = make_float2(far ? __fadd_ru(__fmul_rn(m, c), -kLift<T>) : ref, l);
+    float2 ml = make_float2(far ? m * c : ref, l);
     if (m <= floor && l < 0.5f) ml = make_float2(-INFINITY, 0.f);
     // The sums go where Q and the ring were: the first stream's to Q's place (all scores have been multiplied when its last product is
     // done), the second's behind it (everything has); where the streams' number of tiles differs, when both are done. Pieces of 16 bytes,

@@ -263,13 +263,13 @@ def test_attention_scores_far_beyond_their_differences(cuda_ctx, kind, spread, B
 
 
 @pytest.mark.parametrize("B,kvH,G,d,P,cap", [(2, 8, 4, 64, 300, 60), (5, 8, 4, 64, 9000, 100), (24, 8, 4, 128, 1500, 40), (70, 2, 8, 40, 2500, 60), (200, 8, 4, 64, 1500, 30), (3, 2, 2, 256, 700, 9)])
-@pytest.mark.parametrize("kind,low", [("bf16", -3.3895313892515355e38), ("f32", -3.4028234663852886e38), ("f16", -65504.0)])
-def test_attention_rows_with_nothing_but_the_lowest_scores(cuda_ctx, kind, low, B, kvH, G, d, P, cap):
+@pytest.mark.parametrize("kind,low,pick", [("bf16", -3.3895313892515355e38, 1.0), ("f32", -3.4028234663852886e38, 1.0), ("f16", -65504.0, 1.0), ("f16", -65504.0, 32768.0)])
+def test_attention_rows_with_nothing_but_the_lowest_scores(cuda_ctx, kind, low, pick, B, kvH, G, d, P, cap):
     """Keys whose scores are the lowest number that the type has, as a mask leaves them (the query picks one element): where a row has nothing else
     they weigh the same, and where it has others they weigh nothing."""
     s = attn_args(kind, B, kvH * G, kvH, d, P, cap, [cap - b % 7 for b in range(B)], seed=B + d)
     s["q"].zero_()
-    s["q"].view(B, kvH, G, d)[..., 3] = 1.0
+    s["q"].view(B, kvH, G, d)[..., 3] = pick
     for k, v in ((s["kp"], s["vp"]), (s["ko"], s["vo"])):
         k.view(*k.shape[:-1], kvH, d)[..., 3] = low
         v.copy_(v.float().abs().clamp(0.25, 4.0))
