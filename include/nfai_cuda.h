@@ -101,7 +101,7 @@ int nfai_ctx_destroy(nfai_ctx* ctx);
 
 /* Budget, in nanoseconds, of every device-side wait on another rank (exchange words), where a decode step is one
  * resident kernel (nfai_step_kernels), of its CTAs' waits on one another, and of the waits for copies and products in
- * nfai_op_attn_shared and nfai_op_logit_rules (at most 4 seconds). Default one second, or the environment
+ * nfai_op_attn_shared and nfai_op_logit_rules (at most 2 seconds). Default one second, or the environment
  * variable NFAI_WAIT_NS at context creation. A wait that runs out makes the call return NFAI_ERR_TIMEOUT; the kernel
  * itself always returns, and the cache row of that step is not valid (nfai_set_position goes back). Takes effect for
  * graphs captured afterwards (nfai_model_finalize, nfai_model_tune) and for the next resident step.
@@ -426,9 +426,9 @@ int nfai_rope_frequencies(uint32_t dims, double base, int scaling, double factor
  * multiplied by `magnitude`, the rest and the values as they are; queries into q_out [rows][qH*d], keys and values into rows of
  * k_cache and v_cache [cache_rows][kvH*d]. x holds rows of x_stride elements (0: tightly packed), of which the first
  * (qH + 2 kvH) * d are queries, keys and values, as nfai_op_gemm leaves them. x_dtype and out_dtype: NFAI_F32, NFAI_F16 or NFAI_BF16.
- * positions[rows] and slots[rows] (the cache row of each; null: row r goes to cache row r) are device memory. A row whose slot is
+ * freqs[dims/2], positions[rows] and slots[rows] (the cache row of each; null: row r goes to cache row r) are device memory. A row whose slot is
  * outside the cache (negative, for a padded batch) puts its keys and values nowhere. Slots of a call that are the same: it is not
- * said whose rows stay. The angle is formed in 64 bits. qH or kvH may be 0. Outputs do not overlap x.
+ * said whose elements stay. The angle is formed in 64 bits. qH or kvH may be 0. Outputs do not overlap x.
  * replaces: RoPEShader (NFAI.Vulkan.Shaders/RoPEShader.cs:238-271) and the cache write of MatrixMultiplyShader.cs:286-287 for rows. */
 int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stride, uint32_t rows, uint32_t qH, uint32_t kvH, uint32_t d,
                       uint32_t dims, int layout, const double* freqs, float magnitude, const int32_t* positions, const int32_t* slots,
@@ -436,7 +436,7 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
 
 /* Attention of one token of each of B sequences: out[b][h] = sum_t softmax_t(scale q[b][h] . k_t) v_t, where t runs over the `prefix`
  * rows [prefix][kvH*d] that all share and over the first lens[b] of the sequence's own [B][capacity][kvH*d]. The shared rows are read
- * once for all. q and out are [B][qH*d]; everything is of `dtype` (any of the three), scores, weights and sums are float32. For the product
+ * once for all where that pays (not behind short prompts, and not with 16-bit heads above 128: there every sequence reads them). q and out are [B][qH*d]; everything is of `dtype` (any of the three), scores, weights and sums are float32. For the product
  * with the values of 16-bit caches and heads up to 128 a weight is rounded: to the caches' type where the shared rows are walked for all
  * (in float16 to steps of 2^-31 of the row's largest weight at the finest), to two terms of it elsewhere (steps of 2^-39). Which of both
  * depends on the sizes, so a sequence alone and in a batch may differ in the last bit. scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.

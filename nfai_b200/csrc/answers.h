@@ -44,7 +44,7 @@ struct LogitRules {
   uint32_t n_masks = 0;
   const int32_t* mask_rows = nullptr; // [rows]; null: row r has mask r
   uint32_t* err = nullptr;            // device word of the context; may be null
-  uint32_t wait_ns = 1000000000u;     // budget of a wait
+  uint32_t wait_cycles = 2000000000u; // budget of a wait
 };
 cudaError_t launch_logit_rules(cudaStream_t s, const LogitRules& p);
 
@@ -68,7 +68,7 @@ struct SharedAttn {
   uint32_t own_splits = 1, own_least = 64; // parts of a sequence's keys at most, and keys of a part at least
   bool joined = false;                // partial results go to scratch and a last kernel joins them (else the CTAs of a row do, if it has more than one)
   uint32_t* err = nullptr;            // device word of the context; may be null
-  uint32_t wait_ns = 1000000000u;     // budget of a wait
+  uint32_t wait_cycles = 2000000000u; // budget of a wait
 };
 // What the sizes alone decide: which kernels run, into how many parts, and what scratch they need.
 struct SharedPlan {

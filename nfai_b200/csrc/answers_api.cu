@@ -37,7 +37,7 @@ int finish(nfai_ctx* c, void* stream, cudaError_t launched, bool waits) {
   CU(c, cudaMemsetAsync(c->answers_note(), 0, 4, c->stream));
   return fail(c, NFAI_ERR_TIMEOUT, "a bounded device-side wait gave up");
 }
-uint32_t budget(const nfai_ctx* c) { return (uint32_t)(c->wait_ns < 4000000000ull ? c->wait_ns : 4000000000ull); }
+uint32_t budget(const nfai_ctx* c) { return 2 * (uint32_t)(c->wait_ns < 2000000000ull ? c->wait_ns : 2000000000ull); }  // in cycles
 bool known_dtype(int t) { return t == NFAI_F32 || t == NFAI_F16 || t == NFAI_BF16; }
 #define ON_DEVICE(c)                                        \
   if (!(c)) return fail(nullptr, NFAI_ERR_ARG, "ctx is null"); \
@@ -125,7 +125,7 @@ int nfai_op_logit_rules(nfai_ctx* c, const float* logits, uint32_t rows, uint32_
   p.history = history; p.history_stride = history ? history_stride : 0; p.history_len = history_len;
   p.repetition = repetition; p.frequency = frequency; p.presence = presence;
   p.bias_start = bias_start; p.bias_ids = bias_ids; p.bias = bias; p.n_bias = n_bias;
-  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->answers_note(); p.wait_ns = budget(c);
+  p.masks = masks; p.n_masks = n_masks; p.mask_rows = mask_rows; p.err = c->answers_note(); p.wait_cycles = budget(c);
   return finish(c, stream, launch_logit_rules(stream_of(c, stream), p), true);
 }
 
@@ -170,7 +170,7 @@ int nfai_op_attn_shared(nfai_ctx* c, const void* q, const void* k_prefix, const 
   p.pre_o = (float*)(base + plan.pre_o); p.pre_ml = (float*)(base + plan.pre_ml);
   p.own_o = (float*)(base + plan.own_o); p.own_ml = (float*)(base + plan.own_ml);
   p.pre_splits = plan.pre_splits; p.pre_tiles = plan.pre_tiles; p.own_splits = plan.own_splits; p.own_least = plan.own_least; p.joined = plan.joined;
-  p.err = c->answers_note(); p.wait_ns = budget(c);
+  p.err = c->answers_note(); p.wait_cycles = budget(c);
   return finish(c, stream, launch_shared_attn(stream_of(c, stream), dtype, p, plan), true);
 }
 

@@ -2,8 +2,9 @@
 // and over the sequence's own. Reference arithmetic: AttentionScoreCalculationShader.cs:170-205, AttentionSoftmaxShader.cs:145-177,
 // AttentionWeightedValueSumShader.cs:181-215, once per sequence.
 //
-// This file holds the plan of a call, the join and the kernel on the CUDA cores, which serves float32 and heads above 128: a CTA has the query heads of one KV
-// head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
+// This file holds the plan of a call, the join and the kernel on the CUDA cores, which serves float32 and heads above 128 (there, in 16 bits,
+// the shared rows too, for every sequence once more: 64 sequences of 16 over 4 heads of 256 behind 16384 rows 3.7 ms, in float32, whose
+// walk takes such heads, 0.67 ms): a CTA has the query heads of one KV head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
 // (a quarter of the head each, all query heads), then a thread has four of the output's dimensions and every n-th key.
 #include "attn_shared_common.cuh"
 
@@ -274,6 +275,9 @@ __global__ void __launch_bounds__(kJT) attn_shared_join_kernel(const SharedAttn 
 template <typename T, int LANES, int UNITS>
 cudaError_t launch_join_of(cudaStream_t s, const SharedAttn& p) {
   const uint32_t rows = p.B * p.qH;
+  // Four warps a row where there are many parts and CTAs for all of them at once, a warp a row | four: 3 sequences of 16 heads of 128 behind 100000
+  // rows 29.1 | 22.9 us a call, 8 of 32 of 128 behind 2011 11.5 | 11.0, 5 of 32 of 64 behind 100003 40.7 | 40.5, in float32 9 of 8 of 32 behind 1000
+  // 8.6 | 8.5; 64 of 32 of 128 behind 32768 (2048 rows, 18 parts) 67.8 | 69.7.
   if (p.pre_splits + p.own_splits > 16 && rows < 148 * 32)
     return launch_pdl(attn_shared_join_kernel<T, 4, LANES, UNITS>, dim3(rows), dim3(kJT), 0, s, true, p);
   return launch_pdl(attn_shared_join_kernel<T, 1, LANES, UNITS>, dim3((rows + 3) / 4), dim3(kJT), 0, s, true, p);
@@ -293,9 +297,16 @@ cudaError_t launch_own(cudaStream_t s, const SharedAttn& p, const SharedPlan& pl
 }  // namespace
 
 namespace {
-constexpr uint32_t kLeastOfAll = 32;                                                            // keys of a part of the own rows at least
-constexpr uint32_t own_rows_of(bool tensor, uint32_t G) { return tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8); }  // query heads of a CTA
-constexpr uint32_t own_ctas_of(bool tensor) { return 148 * (tensor ? 2 : 4); }                   // CTAs that the own rows are cut into
+constexpr uint32_t kLeastOfAll = 32;  // keys of a part of the own rows at least
+// Query heads of a CTA. On the tensor cores, 8 | 16: 64 sequences of 32 heads over 8 of 64 with 500 keys 15.5 | 15.9 us, of 8 over 1 with 900 9.2 | 9.4;
+// of 16 over 1 of 128 with 2000 24.4 | 21.9 (16 are two CTAs on the same keys), 40 of 32 over 2 of 64 with 1300 16.7 | 14.0. On the CUDA cores, 4 | 8:
+// 16 of 32 over 8 of 64 with 700 25.9 | 32.1, 20 of 16 over 4 of 256 with 800 97 | 124; of 16 over 2 88 | 49, 30 of 16 over 2 of 64 with 600 28.1 | 21.1.
+constexpr uint32_t own_rows_of(bool tensor, uint32_t G) { return tensor ? (G <= 8 ? 8 : 16) : (G <= 4 ? 4 : 8); }
+// CTAs that the own rows are cut into: two for an SM, on the CUDA cores four. 1 | 2 | 3 | 4: 8 sequences of 32 over 8 heads of 128 with 6000 keys 42.5 |
+// 35.0 | 41.7 | 37.7 us, 4 of 64 with 9000 32.1 | 23.0 | 20.6 | 20.4, 20 of 64 with 1700 25.2 | 19.0 | 17.7 | 16.7, 3 of 16 over 1 of 128 with 20000
+// 15.5 | 16.1 | 18.3 | 18.1. CUDA cores, 1 | 2 | 4 | 8: 4 of 32 over 8 of 64 with 5000 73 | 47 | 43 | 42, 9 of 8 over 2 of 32 behind 1000 10.7 | 9.2 |
+// 8.6 | 8.5, in 16 bits 4 of 16 over 4 of 256 with 3300 67 | 53 | 60 | 59.
+constexpr uint32_t own_ctas_of(bool tensor) { return 148 * (tensor ? 2 : 4); }
 }  // namespace
 
 SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, uint32_t d, uint32_t prefix, uint32_t capacity) {
@@ -331,9 +342,11 @@ SharedPlan plan_shared_attn(int dtype, uint32_t B, uint32_t qH, uint32_t kvH, ui
   const uint64_t keys = (uint64_t)capacity + (shared ? 0 : prefix);
   a.rows = own_rows_of(a.tensor, G);
   const uint64_t groups = (uint64_t)B * kvH * ((G + a.rows - 1) / a.rows);
-  // CTAs for every SM twice over (the CUDA cores' four times) where the keys go so far. A part has 128 keys at least where the walk of the
+  // As many parts as there are CTAs for, where the keys go so far. A part has 128 keys at least where the walk of the
   // shared rows hides the time it takes (8 sequences behind 2011 rows: 11.4 us, 11.9 with 64, 12.3 with 32; 5 behind 100003: 46.3, 45.5,
-  // 44.6), 32 where it is all there is (2 sequences of 340 keys and a join: 5.9 us, 6.2 with 64, 6.1 with 128).
+  // 44.6), 32 where it is all there is (2 sequences of 340 keys and a join: 5.9 us, 6.2 with 64, 6.1 with 128). On the CUDA cores 64, a tile, 32 | 64 |
+  // 128: 9 sequences of 8 over 2 heads of 32 behind 1000 rows 11.5 | 8.5 | 9.6, 2 of 8 over 2 of 64 with 340 keys 7.1 | 7.4 | 9.2, in 16 bits 3 of 16
+  // over 4 of 256 with 1000 25.1 | 19.6 | 18.1.
   a.own_least = !a.tensor ? 64 : shared ? 128 : kLeastOfAll;
   uint64_t parts = (own_ctas_of(a.tensor) + groups - 1) / groups;
   if (parts > (keys + a.own_least - 1) / a.own_least) parts = (keys + a.own_least - 1) / a.own_least;

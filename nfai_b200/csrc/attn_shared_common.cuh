@@ -26,9 +26,9 @@ __device__ __forceinline__ float s_ex2(float x) {
   return y;
 }
 
-// Bounded waits as in umma.cuh, with the context's budget; it is counted in cycles (two a nanosecond), whose counter is read in a few of
-// them (the nanosecond timer takes longer than some of these waits). How long one try may sleep is up to the hardware: with a budget below
-// a millisecond the barrier is asked without sleeping.
+// Bounded waits as in umma.cuh, with the context's budget. It is counted in cycles (two a nanosecond), whose counter is read in a few of
+// them (the nanosecond timer takes longer than some of these waits); 32 bits of it are enough for two seconds. How long one try may sleep is
+// up to the hardware, so the barrier is asked without sleeping first: a budget of a few cycles is kept too.
 __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -40,12 +40,12 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t ns) {
-  const bool sleep = ns >= 1000000u;
-  if (sleep && umma::bar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (sleep ? !umma::bar_try(bar, parity) : !bar_test(bar, parity))
-    if (clock64() - t0 > 2ll * ns) return false;
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint32_t cycles) {
+  if (bar_test(bar, parity)) return true;
+  const uint32_t t0 = clock();
+  do {
+    if ((uint32_t)clock() - t0 > cycles) return false;
+  } while (!umma::bar_try(bar, parity));
   return true;
 }
 // Where one gave up: a millisecond, for copies and products that are on their way to end before their memory is used for something else. (They
@@ -55,7 +55,7 @@ __device__ __forceinline__ void let_land() {
   while (clock64() - t0 < 2000000ll) {
   }
 }
-__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity, uint32_t ns) { return __all_sync(0xffffffffu, wait_for(bar, parity, ns)); }
+__device__ __forceinline__ bool all_wait_for(uint32_t bar, uint32_t parity, uint32_t cycles) { return __all_sync(0xffffffffu, wait_for(bar, parity, cycles)); }
 
 // The walk of one CTA: keys [t0, t1) of sequence b's n, the shared rows first unless they have kernels of their own.
 struct Walk {

@@ -10,8 +10,8 @@
 // they multiply this one's last, spare the joining but not the wait for the warp with one part more: 77 us for 68 with 256 sequences.
 // A weight is split into two 16-bit terms (two products into one sum): the products wait for memory anyway. In float16 22 bits of it count,
 // down to 2^-40 of the row's largest (kLift), in bfloat16 16.
-// 256 sequences of 32 heads of 64 with 500 rows of their own (and 60 shared ones): 44.9 us, 5.9 TB/s; of 128, 64 sequences: 4.4 TB/s (512 CTAs, three
-// to an SM: the second wave is not full).
+// 256 sequences of 32 heads of 64 with 475 rows of their own on average (and 60 shared ones): 44.4 us, 5.6 TB/s; of 128, 64 sequences: 27.9 us,
+// 4.5 TB/s (512 CTAs, three to an SM: the second wave is not full).
 #include "attn_shared_common.cuh"
 
 namespace nfai {
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kMT) attn_shared_mma_kernel(const __grid_const
     const uint32_t cnt = count_of(i);
     __syncwarp();  // every lane is past its reads of the stage that is filled next
     if (i + (NST - 1) * kMW < slices && ok) issue(i + (NST - 1) * kMW);
-    ok = __all_sync(0xffffffffu, ok && wait_for(full + 8 * use, phase, p.wait_ns));
+    ok = __all_sync(0xffffffffu, ok && wait_for(full + 8 * use, phase, p.wait_cycles));
     const uint32_t ks = ring + use * 2 * SH::kHalf, vs = ks + SH::kHalf;
     if (cnt < kSlice) {
       unsigned char* const v = stages + (use * 2 + 1) * SH::kHalf;

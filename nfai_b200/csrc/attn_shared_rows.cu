@@ -8,8 +8,9 @@
 // the SM's other CTAs, of which two buffers leave room for fewer (50 sequences of 6 heads of 128 behind 3800 rows: 44.7 us with two buffers,
 // 32.9 with one; 36 of 16 of 64 behind 4000: 76.3 and 72.4). Partial results go to scratch as those of attn_shared_umma.cu.
 //
-// Bound by the multiply-add units and the loads that feed them: 15 to 18 TFLOP/s for the whole call with 36 rows and more of a KV head (9
-// sequences of 32 heads of 64 behind 8000 rows: 40 us; 50 of 6 heads of 128 behind 3800: 33 us), where one sequence after another takes 123 us.
+// 15 to 18 TFLOP/s for the whole call with 36 rows and more of a KV head, a quarter of what the multiply-add units do (9 sequences of 32 heads of
+// 64 behind 8000 rows: 43 us; 50 of 6 heads of 128 behind 3800: 33 us, where one sequence after another takes 123). Bound by waiting: a tile is
+// fetched, then used, ten warps an SM issue in 42 % of the cycles, and what they wait for is the units' and shared memory's latency.
 #include "attn_shared_common.cuh"
 
 namespace nfai {

@@ -6,9 +6,10 @@
 // neighbouring row tiles on the same keys, which are then fetched once for 256 rows; with fewer they are the same rows on every second
 // tile of keys. While one stream forms its weights the tensor pipe works for the other:
 //   warp 16  K and V tiles by TMA into a ring of 128-byte swizzled slots, in the order in which they are multiplied
-//   warp 17  one lane issues S(0), S(1), then for every unit (stream, tile) u: O += P(u) V, S(u + 2) = Q K^T, with P in tensor memory where S(u)
-//            was (for heads up to 64 there is room for a third unit: S(u + 3)) and V as it lies (its rows run along N). (A warp for each stream was no faster, 76 us for 72 with 64 sequences behind 32768
-//            rows: the streams fell into step and wanted the same units at the same time.)
+//   warp 17  one lane issues S(0), S(1), then for every unit (stream, tile) u: O += P(u) V, S(u + 2) = Q K^T, with P in tensor memory where
+//            S(u) was (for heads up to 64 there is room for a third unit: S(u + 3)) and V as it lies (its rows run along N). (A warp for
+//            each stream was no faster, 76 us for 72 with 64 sequences behind 32768 rows: the streams fell into step and wanted the same
+//            units at the same time.)
 //   warp 18  sees the ring's slots fill, in order, and arrives with the softmax warps on the barrier that warp 17 waits for: waiting for the
 //            tiles itself cost that warp 600 of 3700 cycles in which nothing was multiplied
 //   warps 0-7 and 8-15  softmax of a stream, two threads to a row (64 keys each): weights back into tensor memory as the 16-bit
@@ -17,11 +18,13 @@
 // for the others: a row's exponentials are then spread over the schedulers, whose warps each see 32 lanes only.
 // At the end sums of weighted values, maxima and sums of weights go to scratch line by line, by way of shared memory, where streams and
 // copies of the same rows are joined; attn_shared_join_kernel joins the parts with those of the own rows.
-// Bound by the softmax warps: a tile of 128 keys takes them 1850 cycles, of which the unit for exponentials works 1024. A fourth of the weights
-// is computed as a polynomial for that reason. 128 sequences of 32 heads of 64 behind 20000 rows: 48.4 us, with a third unit 45.6, with the
-// polynomial 44.2 (for an eighth of the weights 44.4, a third 45.0); 64 of 32 of 128 behind 32768: 68.9, polynomial 68.2. For those the
-// kernel itself takes 42 us, 0.82 PFLOP/s, where 1.68 have been measured: the two products of a tile take 1290 cycles, 4 us at the end
-// are the sums' way to memory. With few rows it is bound by memory: 5 sequences of 32 heads of 64 behind 100003 rows 40 us, 5.1 TB/s.
+// Bound by what a stream's tile takes one after the other: a tile of 128 keys takes the softmax warps 1850 cycles (scores from tensor memory,
+// maximum and first half of the weights 900, second half 790, the way back 150; the unit for exponentials works 768 of them, 1024 without the
+// fourth of the weights that is computed as a polynomial), the two products 1290 more, of which the other stream's softmax covers a part; no
+// unit is busy for more than half of the time. 128 sequences of 32 heads of 64 behind 20000 rows: 48.4 us, with a third unit 45.6, with the
+// polynomial 43.5 (for an eighth of the weights 43.7, a third 44.3), 44.5 since scores and values of any size are looked after. 64 of 32 of 128
+// behind 32768: 67.6, and 69.0; the kernel itself takes 40 us, 0.85 PFLOP/s, where 1.68 have been measured; 4 us at its end are the
+// sums' way to memory. With few rows it is bound by memory: 5 sequences of 32 heads of 64 behind 100003 rows 40 us, 5.2 TB/s.
 // Weights are rounded to the caches' type, as the product takes both operands of one type and a second term would double its time: a result is
 // 1.05 to 1.4 times as far from the one in 64 bits as with weights of 32, where the rounding of the result is nearly all.
 // Scores are products of the 16-bit queries as they are; the scale goes into the exponent's multiply-add. A row's sums are rescaled only
@@ -40,6 +43,7 @@ using namespace umma;
 using shared_attn::all_wait_for;
 using shared_attn::kPreRows;
 using shared_attn::kPreTile;
+using shared_attn::s_ex2;
 using shared_attn::wait_for;
 
 constexpr int kSoftmax = 512, kThreads = kSoftmax + 96;
@@ -66,11 +70,6 @@ struct PreSmem {
 static_assert(PreSmem<64>::kTotal <= 232448 && PreSmem<128>::kTotal <= 232448, "shared memory of a CTA");
 static_assert(2 * kPreRows * 64 * 4 <= PreSmem<64>::kBarOff && 2 * kPreRows * 128 * 4 <= PreSmem<128>::kBarOff, "both streams' sums go where Q and the ring were");
 
-__device__ __forceinline__ float p_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 2^x of two numbers (x up to 127, NaN stays NaN, below -126.5 gives 0) without the unit for it: x = n + f with a whole n and f in
 // [-1/2, 1/2], 2^f as a polynomial of degree 5 (fitted to the least relative error by weighted least squares on Chebyshev points; in
 // float32 off by 2.2e-7 at most), and 2^n put together from its exponent.
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     uint32_t j = 0;
     auto load = [&](const CUtensorMap* map, uint32_t it) {
       const uint32_t s = j % SM::kSlots;
-      if (j >= SM::kSlots && !all_wait_for(empty0 + 8 * s, (j / SM::kSlots - 1) & 1, p.wait_ns)) return ok = false;
+      if (j >= SM::kSlots && !all_wait_for(empty0 + 8 * s, (j / SM::kSlots - 1) & 1, p.wait_cycles)) return ok = false;
       if (elect_one()) {
         bar_expect_tx(full0 + 8 * s, SM::kTile);
 #pragma unroll
@@ -203,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         if (!load(&mapK, it) || !load(&mapV, it)) break;
     }
     // the last slots' products, as drain_ring does, within the budget
-    for (uint32_t i = j > SM::kSlots ? j - SM::kSlots : 0; i < j && ok; ++i) ok = all_wait_for(empty0 + 8 * (i % SM::kSlots), i / SM::kSlots & 1, p.wait_ns);
+    for (uint32_t i = j > SM::kSlots ? j - SM::kSlots : 0; i < j && ok; ++i) ok = all_wait_for(empty0 + 8 * (i % SM::kSlots), i / SM::kSlots & 1, p.wait_cycles);
   } else if (warp == 17) {
     // 16-bit operands, float32 sums; A along K in both products; B along K (K tile) or along N (V tile)
     constexpr uint32_t idesc_s = kTypes | ((kPreTile >> 3) << 17) | ((kPreRows >> 4) << 24);
@@ -225,12 +224,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         umma_commit(s_ready(u));
       }
     };
-    ok = all_wait_for(q_ready, 0, p.wait_ns);  // Q, and the first keys' tiles
+    ok = all_wait_for(q_ready, 0, p.wait_cycles);  // Q, and the first keys' tiles
     fence_after();
     for (uint32_t u = 0; u < NB && u < units && ok; ++u) scores(u);
     for (uint32_t u = 0; u < units && ok; ++u) {
       const uint32_t st = u & 1, it = u >> 1, j = values_of(u);  // it: the stream's own count
-      if (!(ok = all_wait_for(p_ready(u), p_turn(u), p.wait_ns))) break;  // the weights, the values' tile and the next scores' keys
+      if (!(ok = all_wait_for(p_ready(u), p_turn(u), p.wait_cycles))) break;  // the weights, the values' tile and the next scores' keys
       fence_after();
       if (elect_one()) {
         const uint32_t s = j % SM::kSlots, v_s = base + SM::kRing + s * SM::kTile;
@@ -249,13 +248,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     const uint32_t tiles = 2 * n;
     uint32_t seen = 0;
     auto see = [&](uint32_t upto) {  // the first `upto` tiles have arrived
-      for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1, p.wait_ns);
+      for (; seen < upto && ok; ++seen) ok = all_wait_for(full0 + 8 * (seen % SM::kSlots), (seen / SM::kSlots) & 1, p.wait_cycles);
     };
     see(min(tiles, twice ? NB : (NB - 1) / 2 * 2 + 1));
     if (ok && lane == 0) bar_arrive(q_ready);
     for (uint32_t u = 0; u < units && ok; ++u) {
       see(min(tiles, twice ? 2 * u + NB + 2 : (u + NB) / 2 * 2 + 1));
-      if (u >= NB && ok) ok = all_wait_for(p_ready(u), p_turn(u - NB), p.wait_ns);  // (the phase before has ended: this arrival is for the next)
+      if (u >= NB && ok) ok = all_wait_for(p_ready(u), p_turn(u - NB), p.wait_cycles);  // (the phase before has ended: this arrival is for the next)
       if (ok && lane == 0) bar_arrive(p_ready(u));
     }
   } else {
@@ -300,12 +299,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     // has a ref of this kind, and its neighbours keep their bits.)
     // floor: the lowest score that times c is a number, so that every such score counts.
     float m = floor, ref = 0.f, l = 0.f;
-    bool far = false, any_far = false;
+    bool far = false;
     for (uint32_t it = 0; it < tiles; ++it) {
       // These scores are there, and the products that were issued before them are done: with NB = 2 that of this stream's last tile is
       // one of them, with NB = 3 that of the tile before. (A warp that gave up still meets the other one.)
       const uint32_t u = 2 * it + st, cS = u % NB * kSP;
-      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(u), s_turn(u), p.wait_ns));
+      ok = __all_sync(0xffffffffu, ok && wait_for(s_ready(u), s_turn(u), p.wait_cycles));
       if (!there) {
         __syncwarp();
         if (lane == 0) bar_arrive(p_ready(u));
@@ -341,13 +340,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           const bool was_far = far;
           ref = __fadd_ru(__fmul_ru(top, c), -kLift<T>);
           far = fabsf(ref) > kFar;
-          any_far = __any_sync(0xffffffffu, far);
           if (far) ref = 0.f;  // (and no lift: what a part hands on could not be lower by it)
           if (it) {
             const float lifted = far == was_far ? 0.f : far ? -kLift<T> : kLift<T>;
-            const float f = p_ex2(far || was_far ? (m - top) * c + lifted : before - ref);
+            const float f = s_ex2(far || was_far ? (m - top) * c + lifted : before - ref);
             l *= f;
-            if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1, p.wait_ns));
+            if (NB > 2) ok = __all_sync(0xffffffffu, ok && wait_for(pv_done(st), (it - 1) & 1, p.wait_cycles));
             fence_after();
 #pragma unroll 1
             for (uint32_t k = half * (D / 2); k < (half + 1) * (D / 2); k += 16) {
@@ -361,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
           m = top;
         }
         sum[0] = sum[1] = 0;
-        if (any_far) {
+        if (__any_sync(0xffffffffu, far)) {
           const float less = far ? m : 0.f;
 #pragma unroll
           for (uint32_t j = 0; j < kMine; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) - less);
@@ -375,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
             if (j % 4 == 3) {
               poly_ex2(a, b);
             } else {
-              a = p_ex2(a);
-              b = p_ex2(b);
+              a = s_ex2(a);
+              b = s_ex2(b);
             }
             sum[j & 1] = add2(sum[j & 1], pair(a, b));
             w[j] = pack2(a, b, T());
@@ -410,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
       __syncwarp();
       if (lane == 0) bar_arrive(p_ready(u));
     }
-    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_last(st), 0, p.wait_ns));
+    if (tiles) ok = __all_sync(0xffffffffu, ok && wait_for(pv_last(st), 0, p.wait_cycles));
     if (there) {
       swap[half * kPreRows + place] = l;
       meet();
@@ -458,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (uint32_t k = 0; k < 2 * COPIES; ++k) {
-          f[k] = f[k] == -INFINITY ? 0.f : p_ex2(f[k] - top);
+          f[k] = f[k] == -INFINITY ? 0.f : s_ex2(f[k] - top);
           const float lk = mls[from(k) + kPreRows];
           if (f[k] != 0.f || lk != lk) {
             const float4 v = *reinterpret_cast<const float4*>(sm + (k / COPIES) * (kPreRows * D * 4) + piece((k % COPIES) * kLanesOf + r, e));

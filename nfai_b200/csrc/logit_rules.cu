@@ -13,12 +13,13 @@
 // The mask comes last: a lane has the bits of 32 tokens, which the warp then takes one lane's after the other, so that neighbouring lanes
 // write neighbouring tokens.
 // 48 rows of 128256: 9.5 us with nothing asked for (5.2 TB/s), 14.5 with 4000 tokens of history, 12.4 with a mask for every row (17.0 where a
-// thread had four neighbouring tokens: stores to the same banks), 16.6 with history, biases, and masks for half of the rows: issue slots for
-// the history in every slice are what it costs. Tried: 16 tokens of the history asked for at once (17.5 for 17.1), penalties where
+// thread had four neighbouring tokens: stores to the same banks), 17.0 with history, biases, and masks for half of the rows. Bound by waiting:
+// a CTA walks a chain of steps (lengths, history, counts, penalties, biases, mask, store) while its copy has long arrived and its store has
+// not begun; issue slots are used in 48 % of the cycles, DRAM to less than half of its rate. Tried: 16 tokens of the history asked for at once (17.5 for 17.1), penalties where
 // the logits are stored (22.3: nearly every warp has a touched token and takes the path for all), one wave of slices twice as long
 // with the logits in registers (18.5), clusters of eight slices that share the history and add to one another's counts (21.7: 14.2 with
-// nothing asked for), a look at every token's count a second time (19.1), a plain copy and behind
-// it a CTA a row that has the touched tokens in a hash table (26.2).
+// nothing asked for), a look at every token's count a second time (19.1), a plain copy and behind it a CTA a row that has the touched
+// tokens in a hash table (26.2).
 //
 // In front of SamplingUtils.TopP (NFAI.Models.Llama3/SamplingUtils.cs:5-33); the reference has no such rules.
 #include "answers.h"
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kLT) logit_rules_kernel(const LogitRules p, co
     if (t < len) atomicAdd(count + t, 1u);
   }
   if (front && peel) in_front([&](uint32_t c, uint32_t) { atomicAdd(count + c, 1u); });
-  const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0, p.wait_ns));  // the slice is there, and everything is counted
+  const bool ok = __syncthreads_and(!whole || shared_attn::wait_for(bar, 0, p.wait_cycles));  // the slice is there, and everything is counted
   if (n_hist) {
     auto rule = [&](uint32_t c, uint32_t t) {  // whoever finds a count takes it and leaves none
       const uint32_t n = atomicExch(count + c, 0u);
