@@ -436,10 +436,11 @@ int nfai_op_rope_rows(nfai_ctx* ctx, const void* x, int x_dtype, uint64_t x_stri
 
 /* Attention of one token of each of B sequences: out[b][h] = sum_t softmax_t(scale q[b][h] . k_t) v_t, where t runs over the `prefix`
  * rows [prefix][kvH*d] that all share and over the first lens[b] of the sequence's own [B][capacity][kvH*d]. The shared rows are read
- * once for all where that pays (not behind short prompts, and not with 16-bit heads above 128: there every sequence reads them). q and out are [B][qH*d]; everything is of `dtype` (any of the three), scores, weights and sums are float32. For the product
- * with the values of 16-bit caches and heads up to 128 a weight is rounded: to the caches' type where the shared rows are walked for all
- * (in float16 to steps of 2^-31 of the row's largest weight at the finest), to two terms of it elsewhere (steps of 2^-39). Which of both
- * depends on the sizes, so a sequence alone and in a batch may differ in the last bit. scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
+ * once for all where that pays (not behind short prompts, and not with 16-bit heads above 128: there every sequence reads them). q and
+ * out are [B][qH*d]; everything is of `dtype` (any of the three), scores, weights and sums are float32. For the product with the values of
+ * 16-bit caches and heads up to 128 a weight is rounded: to the caches' type where the shared rows are walked for all (in float16 light
+ * ones to multiples of 2^-31 of the row's largest), to two terms of it elsewhere (multiples of 2^-39). Which of both depends on the sizes,
+ * so a sequence alone and in a batch may differ in the last bit. scale 0 means 1 / sqrt(d). d: a multiple of 8 up to 256.
  * lens (device memory): more than capacity counts as capacity; negative means that the place in the batch is free, and its row
  * of out stays as it was. A sequence without any rows gets zeros; one whose scores are all -infinity gets NaN. An infinite value gives an
  * infinity of its sign to every row that has a weight for it (above 2^-126 of the row's largest), values of both infinities or a NaN give NaN;

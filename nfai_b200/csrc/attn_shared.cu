@@ -4,8 +4,9 @@
 //
 // This file holds the plan of a call, the join and the kernel on the CUDA cores, which serves float32 and heads above 128 (there, in 16 bits,
 // the shared rows too, for every sequence once more: 64 sequences of 16 over 4 heads of 256 behind 16384 rows 3.7 ms, in float32, whose
-// walk takes such heads, 0.67 ms): a CTA has the query heads of one KV head (up to 8) of one sequence and a part of its keys, 64 at a time as float32 in shared memory. Four threads share a key's scores
-// (a quarter of the head each, all query heads), then a thread has four of the output's dimensions and every n-th key.
+// walk takes such heads, 0.67 ms): a CTA has the query heads of one KV head (up to 8) of one sequence and a part of its keys, 64 at a time
+// as float32 in shared memory. Four threads share a key's scores (a quarter of the head each, all query heads), then a thread has four of
+// the output's dimensions and every n-th key.
 #include "attn_shared_common.cuh"
 
 namespace nfai {

@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
     };
     // m: the maximum that counts, of the scores as they are; ref: what their exponents are taken from, an addend of the multiply-add. Both this
     // and the limit on growth are rounded such that no weight is above 2^(kGrowth + kLift). far: the row's ref is so large that its last bit
-    // counts; the maximum is then taken from the scores before they are multiplied. (Row by row: a row of no numbers
-    // has a ref of this kind, and its neighbours keep their bits.)
+    // counts; the maximum is then taken from the scores before they are multiplied. (Row by row: a row of no numbers has a ref of this kind,
+    // and its neighbours keep their bits.)
     // floor: the lowest score that times c is a number, so that every such score counts.
     float m = floor, ref = 0.f, l = 0.f;
     bool far = false;
@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_umma_kernel(const __g
 template <typename T, int D, int COPIES>
 cudaError_t launch_copies(cudaStream_t s, const SharedAttn& p) {
   CUtensorMap mapQ{}, mapK, mapV;
-  if (!encode_cache_map16(&mapK, p.kp, 1, p.prefix, p.kvH, p.d, 64, kPreTile) || !encode_cache_map16(&mapV, p.vp, 1, p.prefix, p.kvH, p.d, 64, kPreTile)) return cudaErrorInvalidValue;
+  if (!encode_cache_map16(&mapK, p.kp, 1, p.prefix, p.kvH, p.d, 64, kPreTile) || !encode_cache_map16(&mapV, p.vp, 1, p.prefix, p.kvH, p.d, 64, kPreTile))
+    return cudaErrorInvalidValue;
   const uint32_t G = p.qH / p.kvH;
   if (kPreRows / COPIES % G == 0 && !encode_query_map16(&mapQ, p.q, p.B, p.kvH, G, p.d, kPreRows / COPIES / G)) return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(attn_shared_umma_kernel<T, D, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PreSmem<D>::kTotal);

@@ -15,11 +15,11 @@
 // 48 rows of 128256: 9.5 us with nothing asked for (5.2 TB/s), 14.5 with 4000 tokens of history, 12.4 with a mask for every row (17.0 where a
 // thread had four neighbouring tokens: stores to the same banks), 17.0 with history, biases, and masks for half of the rows. Bound by waiting:
 // a CTA walks a chain of steps (lengths, history, counts, penalties, biases, mask, store) while its copy has long arrived and its store has
-// not begun; issue slots are used in 48 % of the cycles, DRAM to less than half of its rate. Tried: 16 tokens of the history asked for at once (17.5 for 17.1), penalties where
-// the logits are stored (22.3: nearly every warp has a touched token and takes the path for all), one wave of slices twice as long
-// with the logits in registers (18.5), clusters of eight slices that share the history and add to one another's counts (21.7: 14.2 with
-// nothing asked for), a look at every token's count a second time (19.1), a plain copy and behind it a CTA a row that has the touched
-// tokens in a hash table (26.2).
+// not begun; issue slots are used in 48 % of the cycles, DRAM to less than half of its rate. Tried: 16 tokens of the history asked for at
+// once (17.5 for 17.1), penalties where the logits are stored (22.3: nearly every warp has a touched token and takes the path for all), one
+// wave of slices twice as long with the logits in registers (18.5), clusters of eight slices that share the history and add to one
+// another's counts (21.7: 14.2 with nothing asked for), a look at every token's count a second time (19.1), a plain copy and behind it a
+// CTA a row that has the touched tokens in a hash table (26.2).
 //
 // In front of SamplingUtils.TopP (NFAI.Models.Llama3/SamplingUtils.cs:5-33); the reference has no such rules.
 #include "answers.h"
